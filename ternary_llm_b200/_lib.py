@@ -79,6 +79,14 @@ SIGNATURES = {
     "tllm_b200_matrix_scan": (_int, [_int, _int] + [_vp] * 6 + [ctypes.c_float, _vp, _vp] + [_int] * 7 + [_vp]),
     "tllm_b200_gated_norm": (_int, [_int] + [_vp] * 4 + [_int] * 3 + [ctypes.c_float] * 2 + [_int, _vp]),
     "tllm_b200_experts": (_int, [_int] + [_vp] * 5 + [_int] * 6 + [_vp]),
+    # include/tllm_b200_cache4.h
+    "tllm_b200_rotary_frequencies": (_int, [_int, ctypes.c_double] + [_vp] * 3),
+    "tllm_b200_rotary_turns": (_int, [_vp, _int, _vp]),
+    "tllm_b200_rotary": (_int, [_int, _vp, _vp, _int, _vp, _vp, _int, _vp, _vp, _int, _int, _int, _vp]),
+    "tllm_b200_cache4_append": (_int, [_vp, _int, _vp, _vp, _vp, _int, _vp, _vp, _int, _vp, _vp, _vp]),
+    "tllm_b200_cache4_read": (_int, [_vp, _int, _vp, _vp, _int, _vp, _vp, _vp]),
+    "tllm_b200_cache4_attention": (_int, [_vp, _int, _vp, _vp, _int, _vp, _vp, _int, ctypes.c_float, _int, _int, _vp, ctypes.c_size_t, _vp]),
+    "tllm_b200_cache4_workspace": (_int, [_vp] + [_int] * 4 + [_vp]),
 }
 
 TENSORS_PER_LAYER = 43      # TLLM_T_COUNT
@@ -130,6 +138,26 @@ class MixedDesc(ctypes.Structure):
                [(n, _int) for n in ("loop_start", "loop_stop", "loop_times", "loop_inject")] + \
                [("norm_after_sum", _int), ("residual_scale", ctypes.c_float), ("logit_softcap", ctypes.c_float)] + \
                [("embedding", _vp), ("head", _vp), ("final_norm", _vp), ("layers", ctypes.POINTER(MixedLayerDesc))]
+
+
+class RotaryScaling(ctypes.Structure):
+    """tllm_b200_rotary_scaling (include/tllm_b200_cache4.h)."""
+    _fields_ = [("type", _int)] + [(n, ctypes.c_double) for n in ("factor", "original", "low", "high")]
+
+
+class RotaryTableDesc(ctypes.Structure):
+    """tllm_b200_rotary_table."""
+    _fields_ = [("turns", _vp), ("rot_dim", _int), ("half_layout", _int), ("amplitude", ctypes.c_float)]
+
+
+class Cache4Desc(ctypes.Structure):
+    """tllm_b200_cache4."""
+    _fields_ = [(n, _vp) for n in ("k_codes", "k_params", "v_codes", "v_params")] + [(n, _int) for n in ("batch", "kv_heads", "rows", "dim")]
+
+
+class HeadsDesc(ctypes.Structure):
+    """tllm_b200_heads."""
+    _fields_ = [("p", _vp), ("ld", ctypes.c_longlong)]
 
 
 class TllmError(RuntimeError):

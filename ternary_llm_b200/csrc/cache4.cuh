@@ -1,0 +1,114 @@
+// The 4-bit key/value cache: its layout, the sequences of a call, rotary angles; launchers of
+// rotary.cu, cache4_rows.cu and cache4_attention.cu.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "tllm_b200_cache4.h"
+
+namespace tllm {
+
+using bf16 = __nv_bfloat16;
+
+constexpr int kCacheGroup = TLLM_CACHE4_GROUP;
+
+// Rotation of a head's first `rot` entries; turns null: none.
+struct Rotary {
+    const unsigned long long* turns;
+    int rot, half_layout;
+    float amplitude;
+    int inverse;
+};
+
+// Rows of activations: p + row * ld + head * dim.
+template <typename T>
+struct Rows {
+    T* p;
+    long long ld;
+};
+
+struct Cache4 {
+    uint8_t *kc, *vc;
+    half2 *kp, *vp;                    // (s, l)
+    int batch, kv_heads, rows, dim;
+};
+
+// The sequences of a call; what the device holds is cut to the limits of the tensors, see Span.
+struct Seqs {
+    const int *first, *lens;
+    int batch, tokens, rows;           // rows: of the cache
+    int* err;
+};
+
+#ifdef __CUDACC__
+// Sequence b of a call: n activation rows from row0 on at positions len - n .. len - 1.
+struct Span {
+    int row0, n, len;
+    __device__ __forceinline__ int position(int i) const { return len - n + i; }
+};
+__device__ __forceinline__ Span span_of(const Seqs& s, int b, bool report)
+{
+    const int lo = s.first[b], hi = s.first[b + 1], len = s.lens[b];
+    Span r;
+    r.row0 = min(max(lo, 0), s.tokens);
+    r.n = max(min(max(hi, 0), s.tokens) - r.row0, 0);
+    r.len = min(max(len, 0), s.rows);
+    if (report && (lo < 0 || hi > s.tokens || hi < lo || len < 0 || len > s.rows)) atomicExch(s.err, TLLM_ERR_SHAPE);
+    return r;
+}
+// The sequence that a row belongs to, found by one warp: the first whose end lies behind it; s.batch for none.
+__device__ __forceinline__ int seq_of_row(const Seqs& s, int row, int lane)
+{
+    if (row < s.first[0]) return s.batch;
+    for (int b0 = 0; b0 < s.batch; b0 += 32) {
+        const bool behind = b0 + lane < s.batch && row < s.first[b0 + lane + 1];
+        const uint32_t m = __ballot_sync(0xffffffffu, behind);
+        if (m) return b0 + __ffs(m) - 1;
+    }
+    return s.batch;
+}
+
+// Angle of a pair at a position: the position times the turns a position, as 64-bit fractions of a turn,
+// is exact modulo whole turns; its upper 32 bits are the angle to 2^-32 of a turn.
+__device__ __forceinline__ void turn(const Rotary& r, unsigned long long turns, int position, float& c, float& s)
+{
+    const unsigned long long phase = turns * (unsigned long long)(long long)position + 0x80000000ull;
+    sincospif((float)(int)(phase >> 32) * 0x1p-31f, &s, &c);
+    c *= r.amplitude;
+    s *= r.inverse ? -r.amplitude : r.amplitude;
+}
+
+template <typename T> __device__ __forceinline__ float as_float(T x);
+template <> __device__ __forceinline__ float as_float<half>(half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float as_float<bf16>(bf16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float as_float<float>(float x) { return x; }
+template <typename T> __device__ __forceinline__ T as_type(float x);
+template <> __device__ __forceinline__ half as_type<half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ bf16 as_type<bf16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ float as_type<float>(float x) { return x; }
+
+// First element of a row of the cache, in groups of 64 values.
+__device__ __forceinline__ size_t cache_row(const Cache4& c, int b, int g, int row) { return ((size_t)b * c.kv_heads + g) * c.rows + row; }
+#endif
+
+template <typename T>
+int launch_rotary(const Rotary& r, const int* positions, int tokens, Rows<const T> q, Rows<T> q_out, int heads, Rows<const T> k, Rows<T> k_out,
+                  int kv_heads, int dim, cudaStream_t stream);
+template <typename T>
+int launch_cache4_append(const Cache4& c, const Rotary& r, const Seqs& s, Rows<const T> q, Rows<T> q_out, int heads, Rows<const T> k, Rows<const T> v,
+                         cudaStream_t stream);
+template <typename T>
+int launch_cache4_read(const Cache4& c, const Seqs& s, Rows<T> k, Rows<T> v, cudaStream_t stream);
+
+struct Cache4Call {
+    Cache4 c;
+    Seqs s;
+    int heads, max_new, max_len;
+    float scale;
+    void* ws;
+};
+size_t cache4_workspace(const Cache4& c, int tokens, int heads, int max_new, int max_len);
+template <typename T>
+int launch_cache4_attention(const Cache4Call& a, Rows<const T> q, Rows<T> out, cudaStream_t stream);
+
+}  // namespace tllm

@@ -2128,7 +2128,8 @@ int device_error_check(cudaStream_t stream)
         return fail(TLLM_ERR_LAUNCH, "error flag read: %s", cudaGetErrorString(cudaGetLastError()));
     if (flag != 0) {
         cudaMemset(s->misc + 1, 0, sizeof(int));
-        return fail(flag, "a kernel reported status %d (bounded wait expired)", flag);
+        return fail(flag, "a kernel reported status %d (%s)", flag,
+                    flag == TLLM_ERR_SHAPE ? "sequences of a call outside its tensors" : "bounded wait expired");
     }
     return TLLM_OK;
 }
