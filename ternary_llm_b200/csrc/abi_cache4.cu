@@ -1,5 +1,6 @@
 // extern "C" entry points of the 4-bit key/value cache (include/tllm_b200_cache4.h): argument checks
 // and dispatch to rotary.cu, cache4_rows.cu and cache4_attention.cu.
+#include <climits>
 #include <cmath>
 
 #include "cache4.cuh"
@@ -157,9 +158,10 @@ int tllm_b200_cache4_read(const tllm_b200_cache4* cache, int type, const int* fi
     return launch_cache4_read<float>(c, s, out<float>(k), out<float>(v), S(stream));
 }
 
-static int check_heads(const char* fn, const Cache4& c, int heads, int max_new, int max_len)
+static int check_heads(const char* fn, const Cache4& c, int tokens, int heads, int max_new, int max_len)
 {
     if (heads < 1 || heads > kMostHeads || heads % c.kv_heads) return fail(TLLM_ERR_SHAPE, "%s: %d query heads over %d", fn, heads, c.kv_heads);
+    if ((long long)tokens * heads > INT_MAX) return fail(TLLM_ERR_SHAPE, "%s: %d rows of %d heads", fn, tokens, heads);
     if (max_new < 0 || max_len < 0) return fail(TLLM_ERR_SHAPE, "%s: max_new=%d max_len=%d", fn, max_new, max_len);
     return TLLM_OK;
 }
@@ -170,7 +172,7 @@ int tllm_b200_cache4_workspace(const tllm_b200_cache4* cache, int tokens, int he
     Cache4 c;
     int st;
     if (!bytes) return fail(TLLM_ERR_NULL, "cache4_workspace: null pointer");
-    if ((st = check_cache(fn, cache, &c)) || (st = check_heads(fn, c, heads, max_new, max_len))) return st;
+    if ((st = check_cache(fn, cache, &c)) || (st = check_heads(fn, c, tokens, heads, max_new, max_len))) return st;
     if (tokens < 0) return fail(TLLM_ERR_SHAPE, "cache4_workspace: tokens=%d", tokens);
     *bytes = cache4_workspace(c, tokens, heads, max_new, max_len);
     return TLLM_OK;
@@ -184,7 +186,7 @@ int tllm_b200_cache4_attention(const tllm_b200_cache4* cache, int type, const in
     Cache4Call a;
     int st;
     if ((st = check_type(fn, type, false)) || (st = check_cache(fn, cache, &a.c)) || (st = check_seqs(fn, first, lens, tokens, a.c, &a.s)) ||
-        (st = check_heads(fn, a.c, heads, max_new, max_len)) || (st = check_rows(fn, "q", q, type, tokens, heads, a.c.dim)) ||
+        (st = check_heads(fn, a.c, tokens, heads, max_new, max_len)) || (st = check_rows(fn, "q", q, type, tokens, heads, a.c.dim)) ||
         (st = check_rows(fn, "out", out_rows, type, tokens, heads, a.c.dim)) || (st = check_apart(fn, "q", q, out_rows, type, tokens, heads, a.c.dim)))
         return st;
     if (tokens > 0 && a.c.batch > 0 && q->p == out_rows->p) return fail(TLLM_ERR_SHAPE, "cache4_attention: q overlaps its output");

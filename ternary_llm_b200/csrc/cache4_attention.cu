@@ -2,6 +2,7 @@
 #include <cfloat>
 
 #include "cache4.cuh"
+#include "cache4_work.cuh"
 #include "launch.cuh"
 
 namespace tllm {
@@ -72,12 +73,19 @@ cache4_attention_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T>
 
 }  // namespace
 
-size_t cache4_workspace(const Cache4&, int, int, int, int) { return 0; }
+static bool takes_step(const Cache4& c, int tokens, int heads, int max_new) { return (max_new > 0 ? max_new : tokens) * (heads / c.kv_heads) <= 16; }
+
+size_t cache4_workspace(const Cache4& c, int tokens, int heads, int max_new, int max_len)
+{
+    return takes_step(c, tokens, heads, max_new) ? step_plan(c, tokens, heads, max_new, max_len).bytes : 0;
+}
 
 template <typename T>
 int launch_cache4_attention(const Cache4Call& a, Rows<const T> q, Rows<T> out, cudaStream_t stream)
 {
     if (a.s.tokens == 0 || a.s.batch == 0) return TLLM_OK;
+    if (takes_step(a.c, a.s.tokens, a.heads, a.max_new))
+        return launch_cache4_step<T>(a, q, out, step_plan(a.c, a.s.tokens, a.heads, a.max_new, a.max_len), stream);
     return launch_pdl("cache4_attention", a.c.dim == 64 ? cache4_attention_kernel<T, 64> : cache4_attention_kernel<T, 128>,
                       dim3(a.s.tokens, (a.heads + kWarps - 1) / kWarps), dim3(kThreads), 0, stream, a, q, out);
 }

@@ -46,8 +46,8 @@ def rotate(x, positions, frequencies, amplitude, half):
     return y
 
 
-def attention(q, k, v, position, scale):
-    """One head: q [n, dim] at `position` [n], k and v [m, dim].  (result, sum of weights times |v|, largest sum of |q k| scale)."""
+def attention(q, k, v, position, scale, v_size):
+    """One head: q [n, dim] at `position` [n], k and v [m, dim].  (result, sum of weights times v_size, largest sum of |q k| scale)."""
     s = q @ k.T * scale
     sees = np.arange(len(k))[None] <= position[:, None]
     reach = np.where(sees, np.abs(q) @ np.abs(k).T * scale, 0).max(-1, initial=0.0)
@@ -56,4 +56,4 @@ def attention(q, k, v, position, scale):
     p = np.where(sees, np.exp(s - np.where(np.isfinite(top), top, 0)), 0)
     total = p.sum(-1, keepdims=True)
     p = p / np.where(total > 0, total, 1)
-    return p @ v, p @ np.abs(v), reach
+    return p @ v, p @ v_size, reach

@@ -246,9 +246,11 @@ def check_attention(c, q, out, before, new, heads, dtype, scale, sequences=None)
         for g in range(c.kv_heads if n and (sequences is None or b in sequences) else 0):
             k, v = (ref.values(ref.unpack(codes[b, g, :m]), params[b, g, :m]) for codes, params in ((kc, kp), (vc, vp)))
             rows = x[at:at + n, g * per:(g + 1) * per].reshape(n * per, c.dim)
-            want, size, reach = ref.attention(rows, k, v, np.repeat(np.arange(a, m), per), scale)
+            middle = ref.values(np.full((m, c.dim), 8), vp[b, g, :m])
+            want, size, reach = ref.attention(rows, k, v, np.repeat(np.arange(a, m), per), scale, np.maximum(np.abs(v), np.abs(v - middle)))
             # weights and values may enter as 11 bits (half a step each), keys too: a score moves by 2^-11 of the sum of its terms' sizes, a
-            # weight and the sum of the weights by that; scores and sums in FP32
+            # weight and the sum of the weights by that; scores and sums in FP32.  Where v enters as s (c - 8) and l + 8 s, the rounded weight
+            # meets the first part, |v - (l + 8 s)|, and the second is FP32
             bound = (2 * 2.0 ** -11 + 2 * (2.0 ** -11 + (c.dim + m) * 2.0 ** -24) * reach[:, None]) * size + HALF_STEP[dtype] * np.abs(want) + TINY[dtype]
             err = np.abs(y[at:at + n, g * per:(g + 1) * per].reshape(n * per, c.dim) - want)
             assert (err <= bound).all(), (b, g, float((err / bound).max()))
