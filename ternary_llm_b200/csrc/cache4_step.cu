@@ -409,7 +409,7 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
             }
         __syncthreads();
         const bool complete = j0 == 0 && j1 == chunks;
-        float* rec = complete ? nullptr : static_cast<float*>(a.ws) + ((size_t)blockIdx.x * 2 + (segment > 0)) * kStepRecord<DIM, St::kRows>;
+        float* rec = complete ? nullptr : static_cast<float*>(a.ws) + ((size_t)blockIdx.x * 2 + (segment > 0)) * kRecord<DIM, St::kRows>;
         for (int e = tid; e < tile_rows * (DIM / 4); e += kThreads) {
             const int r = e / (DIM / 4), c = e % (DIM / 4) * 4;
             float top = -INFINITY;
@@ -442,45 +442,6 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
     }
 }
 
-// The records of a head that several CTAs share, joined in their order.  A CTA a head's rows of a tile.
-template <typename T, int DIM, int NT>
-__global__ void __launch_bounds__(kThreads)
-cache4_join_kernel(const Cache4Call a, const Rows<T> out, const int ctas)
-{
-    using St = Step<DIM, NT>;
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, per = a.heads / a.c.kv_heads;
-    pdl_wait();
-    Work<St::kRows, kStepChunk> work(a.s, per, a.c.kv_heads, false, lane);
-    Work<St::kRows, kStepChunk> items(a.s, per, a.c.kv_heads, true, lane);
-    for (long long item = blockIdx.x; item < items.total; item += gridDim.x) {
-        items.find(item, lane);
-        // first chunk of this item among all chunks
-        long long x0 = work.before(items.b, lane) + items.head * work.units(items.span);
-        for (int i = 0; i < items.tile; i++) x0 += work.chunks_of(items.span, i);
-        const long long x1 = x0 + items.chunks;
-        const int c0 = work.owner(x0, ctas), c1 = work.owner(x1 - 1, ctas);
-        if (c0 == c1) continue;
-        const int tile_rows = min(St::kRows, items.rows - items.tile * St::kRows), r0 = items.tile * St::kRows;
-        for (int e = threadIdx.x; e < tile_rows * (DIM / 4); e += kThreads) {
-            const int r = e / (DIM / 4), col = e % (DIM / 4) * 4;
-            float m = -INFINITY, l = 0.f;
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int c = c0; c <= c1; c++) {
-                const bool later = c == c0 && work.start(c, ctas) < x0;
-                const float* rec = static_cast<const float*>(a.ws) + ((size_t)c * 2 + later) * kStepRecord<DIM, St::kRows>;
-                const float top = fmaxf(m, rec[r]), ref = top == -INFINITY ? 0.f : top, f = exp2_neg(m - ref), w = exp2_neg(rec[r] - ref);
-                const float4 v = *reinterpret_cast<const float4*>(rec + 2 * St::kRows + r * DIM + col);
-                m = top;
-                l = fmaf(rec[St::kRows + r], w, l * f);
-                y = make_float4(fmaf(v.x, w, y.x * f), fmaf(v.y, w, y.y * f), fmaf(v.z, w, y.z * f), fmaf(v.w, w, y.w * f));
-            }
-            const int i = (r0 + r) / per, head = items.head * per + (r0 + r) % per;
-            store_row<T>(out.p + (size_t)(items.span.row0 + i) * out.ld + (size_t)head * DIM + col, y, l, items.span.position(i) >= 0);
-        }
-    }
-}
-
 template <typename T, int DIM, int NT>
 int launch(const Cache4Call& a, Rows<const T> q, Rows<T> out, const StepPlan& p, cudaStream_t stream)
 {
@@ -495,7 +456,7 @@ int launch(const Cache4Call& a, Rows<const T> q, Rows<T> out, const StepPlan& p,
     }
     int st = launch_pdl("cache4_step", cache4_step_kernel<T, DIM, NT>, dim3(p.ctas), dim3(kThreads), St::kSmem, stream, a, q, out, p.whole);
     if (st || p.whole) return st;
-    return launch_pdl("cache4_join", cache4_join_kernel<T, DIM, NT>, dim3(p.items), dim3(kThreads), 0, stream, a, out, p.ctas);
+    return launch_cache4_join<T>(a, out, St::kRows, p.ctas, p.items, stream);
 }
 
 }  // namespace

@@ -5,10 +5,10 @@
 
 namespace tllm {
 
-constexpr int kStepChunk = 32;                       // positions a warp takes at once
-constexpr int kLeastShare = 16;                      // chunks that a CTA takes at least where work is cut
+constexpr int kStepChunk = 32;                       // positions a warp of cache4_step.cu takes at once
+constexpr int kPromptChunk = 128, kPromptRows = 256; // positions and rows a CTA of cache4_prompt.cu takes at once
 // Floats of the part of a tile's rows that one CTA found: maxima, sums, outputs.
-template <int DIM, int ROWS> constexpr int kStepRecord = ROWS * (DIM + 2);
+template <int DIM, int ROWS> constexpr int kRecord = ROWS * (DIM + 2);
 
 struct StepPlan {
     int tiles;                                       // of 8 rows that go through the cache together
@@ -20,11 +20,25 @@ StepPlan step_plan(const Cache4& c, int tokens, int heads, int max_new, int max_
 template <typename T>
 int launch_cache4_step(const Cache4Call& a, Rows<const T> q, Rows<T> out, const StepPlan& p, cudaStream_t stream);
 
+struct PromptPlan {
+    bool whole;
+    int ctas, items;
+    size_t bytes;
+};
+PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int max_len);
+template <typename T>
+int launch_cache4_prompt(const Cache4Call& a, Rows<const T> q, Rows<T> out, const PromptPlan& p, cudaStream_t stream);
+
+// Joins what several of `ctas` CTAs found for one tile of rows; items: about how many tiles there are (cache4_join.cu).
+template <typename T>
+int launch_cache4_join(const Cache4Call& a, Rows<T> out, int rows, int ctas, int items, cudaStream_t stream);
+
 #ifdef __CUDACC__
 // Row r of sequence b and key/value head `head` is query head r % per of the head's, of new token r / per; a tile is R of
 // them.  Units are chunks of positions, or whole tiles.  Members are found by whole warps, every lane with the same result.
 template <int R, int CHUNK>
 struct Work {
+    static constexpr int kLeast = CHUNK == kStepChunk ? 16 : 2;            // chunks that a CTA takes at least where work is cut
     Seqs s;
     int per, kv_heads;
     bool whole;
@@ -58,7 +72,7 @@ struct Work {
     __device__ __forceinline__ int used(int parts) const
     {
         if (whole) return parts;
-        const long long most = total / kLeastShare;
+        const long long most = total / kLeast;
         return most < 1 ? 1 : most < parts ? (int)most : parts;
     }
     __device__ __forceinline__ long long start(int c, int parts) const
