@@ -177,9 +177,9 @@ def read(cache: Cache4, k, v, first, lens) -> None:
 
 
 def attention(cache: Cache4, q, out, first, lens, scale: float | None = None, max_new: int = 0, max_len: int = 0) -> None:
-    """out = softmax(scale q k') v over the positions up to each row's own (scale: dim ** -0.5).  max_new, max_len: about the
-    most rows and positions of a sequence, 0 where the caller does not know; results do not depend on them but for the
-    order of sums.  FP16 or BF16."""
+    """out = softmax(scale q k') v over the positions up to each row's own (scale: dim ** -0.5).  max_new: about the most rows
+    of a sequence, 0 where the caller does not know; results do not depend on it but for the order of sums.  max_len: no
+    sequence holds more positions (0: the cache's rows); workspaces are as large as that needs.  FP16 or BF16."""
     kind, d = _type(q, "q", (torch.float16, torch.bfloat16)), cache._desc()
     tokens, heads = q.shape[:2]
     x, y = _rows(q, q.dtype, "q", tokens, heads, cache.dim), _rows(out, q.dtype, "out", tokens, heads, cache.dim)

@@ -195,11 +195,12 @@ int tllm_b200_cache4_attention(const tllm_b200_cache4* cache, int type, const in
     a.scale = scale;
     a.max_new = max_new;
     a.max_len = max_len;
+    if (max_len > 0 && max_len < a.s.rows) a.s.rows = max_len;
     a.ws = workspace;
     const size_t need = cache4_workspace(a.c, tokens, heads, max_new, max_len);
     if (need && !workspace) return fail(TLLM_ERR_NULL, "cache4_attention: the workspace is null");
     if (workspace_bytes < need) return fail(TLLM_ERR_SIZE, "cache4_attention: a workspace of %zu bytes, the call needs %zu", workspace_bytes, need);
-    if (need && misaligned(workspace, 16)) return fail(TLLM_ERR_ALIGN, "cache4_attention: the workspace must be 16-byte aligned");
+    if (need && misaligned(workspace, 128)) return fail(TLLM_ERR_ALIGN, "cache4_attention: the workspace must be 128-byte aligned");
     if ((st = check_device()) || (st = error_flag(&a.s))) return st;
     if (type == TLLM_FP16) return launch_cache4_attention<half>(a, in<half>(q), out<half>(out_rows), S(stream));
     return launch_cache4_attention<bf16>(a, in<bf16>(q), out<bf16>(out_rows), S(stream));

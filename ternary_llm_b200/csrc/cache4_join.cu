@@ -1,5 +1,8 @@
-// Attention over the 4-bit key/value cache: tiles of rows whose positions several CTAs took, joined in the order of
-// the CTAs from their records (maxima, sums of weights, outputs that are not divided by them).
+// Attention over the 4-bit key/value cache: tiles of rows whose positions several CTAs took, joined from the CTAs'
+// records (maxima, sums of weights, outputs that are not divided by them).
+//
+// A CTA here for each that has the first chunk of a shared tile: weights of all records first, then their outputs, every load independent of the others.  A thread has four channels of
+// a row and every kParts-th record; the parts meet in shared memory.  The order of all sums is fixed.
 #include "cache4.cuh"
 #include "cache4_work.cuh"
 #include "dense.cuh"
@@ -9,61 +12,92 @@ namespace tllm {
 
 namespace {
 
-constexpr int kThreads = 256, kBlockRows = 16;       // rows of a tile that a CTA joins
+constexpr int kThreads = 512;
+template <int ROWS> constexpr int kMostCtas = ROWS <= 16 ? 512 : 160;
 
-template <typename T, int DIM, int ROWS, int CHUNK>
+template <typename T, int DIM, int ROWS>
 __global__ void __launch_bounds__(kThreads)
 cache4_join_kernel(const Cache4Call a, const Rows<T> out, const int ctas)
 {
+    constexpr int kBlock = ROWS <= 16 ? 4 : 32;                            // rows of a CTA
+    constexpr int kElems = kBlock * (DIM / 4), kParts = kElems < kThreads ? kThreads / kElems : 1, kStride = 2 * kRecord<DIM, ROWS>;
+    __shared__ float weight[kBlock][kMostCtas<ROWS>], sums[kBlock];
+    __shared__ float4 parts[kParts > 1 ? kThreads : 1];
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, per = a.heads / a.c.kv_heads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = a.heads / a.c.kv_heads, r0 = blockIdx.y * kBlock;
     pdl_wait();
-    Work<ROWS, CHUNK> work(a.s, per, a.c.kv_heads, false, lane), items(a.s, per, a.c.kv_heads, true, lane);
-    for (long long item = blockIdx.x; item < items.total; item += gridDim.x) {
-        items.find(item, lane);
-        // the chunks of this tile among all
-        long long x0 = work.before(items.b, lane) + items.head * work.units(items.span);
-        for (int i = 0; i < items.tile; i++) x0 += work.chunks_of(items.span, i);
-        const int c0 = work.owner(x0, ctas), c1 = work.owner(x0 + items.chunks - 1, ctas);
-        if (c0 == c1) continue;
-        const int r0 = items.tile * ROWS, from = blockIdx.y * kBlockRows, to = min(min(ROWS, items.rows - r0), from + kBlockRows);
-        const bool later = work.start(c0, ctas) < x0;                      // the first CTA had another tile before
-        for (int e = from * (DIM / 4) + threadIdx.x; e < to * (DIM / 4); e += kThreads) {
-            const int r = e / (DIM / 4), col = e % (DIM / 4) * 4;
-            float m = -INFINITY, l = 0.f;
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int c = c0; c <= c1; c++) {
-                const float* rec = static_cast<const float*>(a.ws) + ((size_t)c * 2 + (c == c0 && later)) * kRecord<DIM, ROWS>;
-                const float top = fmaxf(m, rec[r]), ref = top == -INFINITY ? 0.f : top, f = exp2_neg(m - ref), w = exp2_neg(rec[r] - ref);
-                const float4 v = *reinterpret_cast<const float4*>(rec + 2 * ROWS + r * DIM + col);
-                m = top;
-                l = fmaf(rec[ROWS + r], w, l * f);
-                y = make_float4(fmaf(v.x, w, y.x * f), fmaf(v.y, w, y.y * f), fmaf(v.z, w, y.z * f), fmaf(v.w, w, y.w * f));
+    const Shared4 tile = *entry_of(a.ws, blockIdx.x);
+    const int n = tile.parts, rows = min(min(ROWS, tile.n * per - tile.tile * ROWS) - r0, kBlock);
+    if (n == 0 || rows <= 0) return;
+    const float* rec = record_of<DIM, ROWS>(a.ws, ctas, blockIdx.x, 0);
+    const int first = tile.slot ? kRecord<DIM, ROWS> : 0;
+    const auto at = [&](int i) { return rec + (size_t)i * kStride + (i == 0 ? first : 0); };
+    // four channels of a row
+    const auto store = [&](int r, int col, float4 y) {
+        const int i = (tile.tile * ROWS + r0 + r) / per, head = tile.head * per + (tile.tile * ROWS + r0 + r) % per;
+        store_row<T>(out.p + (size_t)(tile.row0 + i) * out.ld + (size_t)head * DIM + col, y, sums[r], tile.len - tile.n + i >= 0);
+    };
+
+    for (int r = warp; r < rows; r += kThreads / 32) {
+        float m = -INFINITY, l = 0.f;
+        for (int i = lane; i < n; i += 32) m = fmaxf(m, at(i)[r0 + r]);
+        m = warp_max(m);
+        const float ref = m == -INFINITY ? 0.f : m;
+        for (int i = lane; i < n; i += 32) {
+            const float w = exp2_neg(at(i)[r0 + r] - ref);
+            weight[r][i] = w;
+            l = fmaf(at(i)[ROWS + r0 + r], w, l);
+        }
+        l = warp_sum(l);
+        if (lane == 0) sums[r] = l;
+    }
+    __syncthreads();
+    for (int e = tid % (kParts > 1 ? kElems : kThreads); e < rows * (DIM / 4); e += kParts > 1 ? kElems : kThreads) {
+        const int r = e / (DIM / 4), col = e % (DIM / 4) * 4, part = kParts > 1 ? tid / kElems : 0;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int i = part; i < n; i += kParts) {
+            const float4 v = *reinterpret_cast<const float4*>(at(i) + 2 * ROWS + (r0 + r) * DIM + col);
+            const float w = weight[r][i];
+            y = make_float4(fmaf(v.x, w, y.x), fmaf(v.y, w, y.y), fmaf(v.z, w, y.z), fmaf(v.w, w, y.w));
+        }
+        if (kParts > 1) parts[tid] = y;
+        else store(r, col, y);
+    }
+    if (kParts > 1) {
+        __syncthreads();
+        if (tid < rows * (DIM / 4)) {
+            float4 y = parts[tid];
+#pragma unroll
+            for (int i = 1; i < kParts; i++) {
+                const float4 v = parts[tid + i * kElems];
+                y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
             }
-            const int i = (r0 + r) / per, head = items.head * per + (r0 + r) % per;
-            store_row<T>(out.p + (size_t)(items.span.row0 + i) * out.ld + (size_t)head * DIM + col, y, l, items.span.position(i) >= 0);
+            store(tid / (DIM / 4), tid % (DIM / 4) * 4, y);
         }
     }
 }
 
-template <typename T, int ROWS, int CHUNK>
-int launch(const Cache4Call& a, Rows<T> out, int ctas, int items, cudaStream_t stream)
+template <typename T, int ROWS>
+int launch(const Cache4Call& a, Rows<T> out, int ctas, cudaStream_t stream)
 {
-    const auto kernel = a.c.dim == 64 ? cache4_join_kernel<T, 64, ROWS, CHUNK> : cache4_join_kernel<T, 128, ROWS, CHUNK>;
-    return launch_pdl("cache4_join", kernel, dim3(items, (ROWS + kBlockRows - 1) / kBlockRows), dim3(kThreads), 0, stream, a, out, ctas);
+    if (ctas > kMostCtas<ROWS>) return fail(TLLM_ERR_SIZE, "cache4_join: %d parts", ctas);
+    const auto kernel = a.c.dim == 64 ? cache4_join_kernel<T, 64, ROWS> : cache4_join_kernel<T, 128, ROWS>;
+    return launch_pdl("cache4_join", kernel, dim3(ctas, ROWS <= 16 ? ROWS / 4 : ROWS / 32), dim3(kThreads), 0, stream, a, out, ctas);
 }
 
 }  // namespace
 
 template <typename T>
-int launch_cache4_join(const Cache4Call& a, Rows<T> out, int rows, int ctas, int items, cudaStream_t stream)
+int launch_cache4_join(const Cache4Call& a, Rows<T> out, int rows, int ctas, cudaStream_t stream)
 {
-    if (rows == 8) return launch<T, 8, kStepChunk>(a, out, ctas, items, stream);
-    if (rows == 16) return launch<T, 16, kStepChunk>(a, out, ctas, items, stream);
-    return launch<T, kPromptRows, kPromptChunk>(a, out, ctas, items, stream);
+    if (rows == 4) return launch<T, 4>(a, out, ctas, stream);
+    if (rows == 8) return launch<T, 8>(a, out, ctas, stream);
+    if (rows == 16) return launch<T, 16>(a, out, ctas, stream);
+    return launch<T, kPromptRows>(a, out, ctas, stream);
 }
 
-template int launch_cache4_join<half>(const Cache4Call&, Rows<half>, int, int, int, cudaStream_t);
-template int launch_cache4_join<bf16>(const Cache4Call&, Rows<bf16>, int, int, int, cudaStream_t);
+template int launch_cache4_join<half>(const Cache4Call&, Rows<half>, int, int, cudaStream_t);
+template int launch_cache4_join<bf16>(const Cache4Call&, Rows<bf16>, int, int, cudaStream_t);
 
 }  // namespace tllm

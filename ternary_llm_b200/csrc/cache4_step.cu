@@ -1,16 +1,17 @@
 // Attention over the 4-bit key/value cache for few rows a sequence: one token of each, or a few.
 //
-// A key/value head's rows (new tokens times the query heads that share it, up to 8 or 16 at once) go through the
-// cache together on mma.sync: codes become FP16 numbers 0..15 in registers (a mask, and one addition or
-// multiplication for two), and the scales stay outside the products:
-//   s_p,r   = scale sum_groups (s_p c_p . q_r + l_p sum q_r)      positions are the rows of the product, query rows its columns
-//   o_r     = sum_p (w_p,r s_p) (c_p - 8) + sum_p w_p,r (l_p + 8 s_p)      channels are the rows; w s rounded to FP16
-// so a code is never multiplied by its scale, keys enter exactly, and a value's only rounding is that of w s, 11
-// bits of it (with a power of two that follows the largest scale seen, so that small scales do not run out of
-// exponents); it meets the difference from the middle of the group's range.  The second sum is FP32.  Weights come out of the first product as pairs of query rows and go into the
-// second as pairs of positions: movmatrix, an 8 x 8 transposition in registers.
-//
-// The running maximum moves when a score exceeds it by more than 2^8; sums are FP32.
+// A key/value head's rows (new tokens times the query heads that share it, up to 4, 8 or 16 at once) go through the
+// cache together on mma.sync.  With keys k = l + s c and values alike, scales and lowest values stay outside the products:
+//   scores   sum_groups s (c . q) + l sum q   c . q in integers: codes are bytes after one mask (and a shift for every
+//            other one), a query is 16 bits of its largest entry in the group, as two signed bytes in neighbouring columns
+//            of the product (m16n8k32), whose sums are joined exactly.  Positions are the rows of the product.
+//   outputs  sum_p (w s) (c - 8) + sum_p w (l + 8 s)   codes are FP16 numbers after a mask and an addition or
+//            multiplication for two, w s is rounded to FP16 (11 bits of it, with a power of two that follows the largest
+//            scale seen, so that small scales do not run out of exponents) and meets the difference from the middle of the
+//            group's range; the second sum is FP32.  Channels are the rows of the product (m16n8k16), columns the
+//            query rows, or with up to four of them the four for the first and the four for the second group.
+// Weights come out of the first product by position and go into the second as pairs of positions: movmatrix, an 8 x 8
+// transposition in registers.  The running maximum moves when a score exceeds it by more than 2^8; sums are FP32.
 //
 // Work is cut into chunks of 32 positions.  All chunks of a call are one sequence of which every CTA takes an equal
 // part, whatever the lengths; a warp takes every eighth of them, through a ring of its own (cp.async, no barrier).
@@ -31,15 +32,20 @@ namespace {
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr float kSlack = 8.f, kLift = 16.f;
 constexpr int kPad = 8;                                     // floats behind a row of a warp's outputs
+constexpr float kDigits = 32512.f;                          // largest query entry in the integer product: 127 * 256
 
-template <int DIM, int NT>
+template <int DIM, int ROWS>
 struct Step {
-    static constexpr int kRows = 8 * NT, kGroups = DIM / 64;
+    static constexpr int kGroups = DIM / 64;
+    static constexpr int kSets = ROWS / 4;                  // column tiles of the first product: four rows, two digits each
+    static constexpr int kCols = ROWS == 4 ? 1 : ROWS / 8;  // column tiles of the second
     static constexpr int kSlots = 2;
     static constexpr int kCodes = kStepChunk * DIM / 2, kParams = kStepChunk * kGroups * 4;
     static constexpr int kSlot = 2 * (kCodes + kParams);    // keys' codes, values' codes, keys' params, values' params
-    static constexpr int kOut = kRows * (DIM + kPad);       // floats of a warp's outputs
-    static constexpr int kSmem = kWarps * (kSlots * kSlot + (kOut + 2 * kRows) * 4);
+    static constexpr int kOut = ROWS * (DIM + kPad);        // floats of a warp's outputs
+    static constexpr int kSmem = kWarps * (kSlots * kSlot + (kOut + 2 * ROWS) * 4);
+    // row of set n that lane t of a quad has in the sums of the first product
+    static __device__ __forceinline__ int row(int n, int t) { return ROWS == 4 ? t : 8 * (n >> 1) + 2 * t + (n & 1); }
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -53,13 +59,10 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool v
 }
 __device__ __forceinline__ uint32_t bits(half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ half2 halves(uint32_t u) { return *reinterpret_cast<const half2*>(&u); }
-// Nibbles 0, 4 / 1, 5 / 2, 6 / 3, 7 less MID as pairs of FP16 numbers: 1024 + c and 1024 + 16 c are bit patterns.
-template <int MID>
+// Nibbles 0, 4 / 1, 5 / 2, 6 / 3, 7 less 8 as pairs of FP16 numbers: 1024 + c and 1024 + 16 c are bit patterns.
 __device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&h)[4])
 {
-    const half2 one = halves(MID ? 0x64086408u : 0x64006400u), sixteenth = halves(0x2c002c00u);              // 1024 + MID, 1 / 16
-    const half2 off = halves(MID ? 0xd480d480u : 0xd400d400u);                                              // -(64 + MID)
-    static_assert(MID == 0 || MID == 8, "constants above");
+    const half2 one = halves(0x64086408u), sixteenth = halves(0x2c002c00u), off = halves(0xd480d480u);      // 1032, 1 / 16, -72
     const uint32_t v = w >> 8;
     h[0] = bits(__hsub2(halves((w & 0x000f000fu) | 0x64006400u), one));
     h[1] = bits(__hfma2(halves((w & 0x00f000f0u) | 0x64006400u), sixteenth, off));
@@ -70,6 +73,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_u8s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v)
 {
@@ -84,12 +92,12 @@ __device__ __forceinline__ int place(int r) { return r < 4 ? r : r ^ 1; }
 // 16-byte pieces of a row of 64 bytes, exchanged in every other pair of rows for the same reason.
 template <int DIM> __device__ __forceinline__ int swizzle(int row) { return DIM == 128 ? row & 2 : 0; }
 
-template <typename T, int DIM, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+template <typename T, int DIM, int ROWS>
+__global__ void __launch_bounds__(kThreads, ROWS == 16 ? 1 : 2)
 cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out, const bool whole)
 {
-    using St = Step<DIM, NT>;
-    constexpr int GR = St::kGroups;
+    using St = Step<DIM, ROWS>;
+    constexpr int GR = St::kGroups, NS = St::kSets, NC = St::kCols, kStep = kWarps * kStepChunk;
     extern __shared__ __align__(16) uint8_t smem[];
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -101,57 +109,76 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
 
     if (blockIdx.x == 0 && warp == 0)
         for (int b = lane; b < a.s.batch; b += 32) span_of(a.s, b, true);
-    Work<St::kRows, kStepChunk> work(a.s, per, a.c.kv_heads, whole, lane);
+    Work<ROWS, kStepChunk> work(a.s, per, a.c.kv_heads, whole, lane);
     const long long from = work.start(blockIdx.x, gridDim.x), to = work.start(blockIdx.x + 1, gridDim.x);
+    if (!whole && tid == 0) entry_of(a.ws, blockIdx.x)->parts = 0;
     if (from >= to) return;
     work.find(from, lane);
     int segment = 0;
 
     for (long long x = from; x < to; segment++) {
         // ---- the next head's rows and the part of its chunks ----
-        const int chunks = work.chunks, j0 = whole ? 0 : work.offset, j1 = whole ? chunks : (int)min((long long)chunks, j0 + (to - x));
-        const int tile_rows = min(St::kRows, work.rows - work.tile * St::kRows), r0 = work.tile * St::kRows;
+        const int chunks = work.chunks, units = work.kFixed + chunks;
+        const int j0 = whole ? 0 : work.chunk_at(work.offset), j1 = whole ? chunks : work.chunk_at(min((long long)units, work.offset + (to - x)));
+        x += whole ? 1 : units - work.offset;
+        if (j0 == j1) {
+            if (x < to) work.next();
+            continue;
+        }
+        const int r0 = work.tile * ROWS, tile_rows = min(ROWS, work.rows - r0);
         const Span sp = work.span;
-        const size_t base = cache_row(a.c, work.b, work.head, 0);
         const int visible = work.visible;                                  // positions that some row sees
 
-        const auto load = [&](int j, int slot) {
-            const uint32_t at = smem_addr(ring + slot * St::kSlot);
-            const int p0 = j * kStepChunk;
-            constexpr int kPieces = DIM / 32;
-#pragma unroll
-            for (int i = 0; i < kPieces; i++) {
-                const int e = i * 32 + lane, row = e / kPieces, c = e % kPieces;
-                const bool valid = p0 + row < visible;
-                const size_t src = (base + (valid ? p0 + row : 0)) * (DIM / 2) + c * 16;
-                const uint32_t dst = at + row * (DIM / 2) + ((c ^ swizzle<DIM>(row)) * 16);
-                copy_async<16>(dst, a.c.kc + src, valid);
-                copy_async<16>(dst + St::kCodes, a.c.vc + src, valid);
-            }
-            const bool valid = p0 + lane < visible;
-            const size_t src = (base + (valid ? p0 + lane : 0)) * GR;
-            copy_async<4 * GR>(at + 2 * St::kCodes + lane * 4 * GR, a.c.kp + src, valid);
-            copy_async<4 * GR>(at + 2 * St::kCodes + St::kParams + lane * 4 * GR, a.c.vp + src, valid);
-        };
+        // a lane copies the same piece of every (32 / pieces of a row)-th row, and a row's params
+        constexpr int kPieces = DIM / 32, kSpan = 32 / kPieces;
+        const int my_row = lane / kPieces;
+        const size_t first_row = cache_row(a.c, work.b, work.head, 0) + (size_t)(j0 + warp) * kStepChunk;
+        const size_t code = (first_row + my_row) * (DIM / 2) + lane % kPieces * 16, par = (first_row + lane) * GR;
+        const uint8_t *k_src = a.c.kc + code, *v_src = a.c.vc + code;
+        const half2 *kp_src = a.c.kp + par, *vp_src = a.c.vp + par;
+        const uint32_t to_codes = smem_addr(ring) + my_row * (DIM / 2) + ((lane % kPieces) ^ swizzle<DIM>(my_row)) * 16;
+        const uint32_t to_params = smem_addr(ring) + 2 * St::kCodes + lane * 4 * GR;
         int issued = j0 + warp;
+        const auto load = [&](int slot) {
+            if (issued < j1) {
+                const int left = visible - issued * kStepChunk;            // positions behind hold anything: nothing of them is read
+                const bool full = left >= kStepChunk;
+                const uint32_t at = slot * St::kSlot;
 #pragma unroll
-        for (int i = 0; i < St::kSlots - 1; i++, issued += kWarps) {
-            if (issued < j1) load(issued, i);
+                for (int i = 0; i < kPieces; i++) {
+                    const bool valid = full || my_row + i * kSpan < left;
+                    const int off = valid ? i * kSpan * (DIM / 2) : 0;
+                    copy_async<16>(to_codes + at + i * kSpan * (DIM / 2), valid ? k_src + off : a.c.kc, valid);
+                    copy_async<16>(to_codes + at + St::kCodes + i * kSpan * (DIM / 2), valid ? v_src + off : a.c.vc, valid);
+                }
+                const bool valid = full || lane < left;
+                copy_async<4 * GR>(to_params + at, valid ? kp_src : a.c.kp, valid);
+                copy_async<4 * GR>(to_params + at + St::kParams, valid ? vp_src : a.c.vp, valid);
+                k_src += kStep * (DIM / 2);
+                v_src += kStep * (DIM / 2);
+                kp_src += kStep * GR;
+                vp_src += kStep * GR;
+            }
+            issued += kWarps;
             asm volatile("cp.async.commit_group;" ::: "memory");
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < St::kSlots - 1; i++) load(i);
 
-        // ---- the query rows: operands of the first product, sums by group, scales ----
-        uint32_t qf[NT][GR][2][2][2];
-        float qsum[NT][2][GR], col_scale[NT][2];
-        int sees[NT][2], least = INT_MAX;
+        // ---- the query rows: digits for the first product, their sums, what a unit of a digit is worth ----
+        uint32_t qd[NS][GR][2][2];
+        float qsum[NS][GR], unit_q[NS][GR];
+        int sees[NS], least = INT_MAX;
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int r = r0 + 8 * n + g;
-            const bool there = 8 * n + g < tile_rows;
+        for (int n = 0; n < NS; n++) {
+            const int rr = St::row(n, g >> 1), r = r0 + rr;                // columns 2 i and 2 i + 1: digits of a row
+            const bool there = rr < tile_rows;
             const T* qp = q.p + (size_t)(sp.row0 + (there ? r / per : 0)) * q.ld + (size_t)(work.head * per + (there ? r % per : 0)) * DIM;
-            float top = 0.f, f[GR][2][8];
+            float sum[GR], worth[GR];
 #pragma unroll
-            for (int gr = 0; gr < GR; gr++)
+            for (int gr = 0; gr < GR; gr++) {
+                float f[2][8], top = 0.f;
+                bool odd = false;
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
                     uint4 v = make_uint4(0, 0, 0, 0);
@@ -159,66 +186,61 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                     const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        f[gr][w][i] = as_float(e[i]);
-                        top = fmaxf(top, fabsf(f[gr][w][i]));
+                        f[w][i] = as_float(e[i]);
+                        top = fmaxf(top, fabsf(f[w][i]));
+                        odd = odd || !(fabsf(f[w][i]) < INFINITY);
                     }
                 }
-            // BF16 numbers become FP16 ones times a power of two of their row, the largest from 2^14 on
-            float up = 1.f, down = 1.f;
-            if constexpr (sizeof(T) == 2 && !std::is_same<T, half>::value) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = (__float_as_int(top) >> 23) - 127;
-                if (top > 0.f && e < 128) {
-                    const int sh = min(14 - e, 126);
-                    up = __int_as_float((127 + sh) << 23);
-                    down = __int_as_float((127 - sh) << 23);
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    odd = __shfl_xor_sync(0xffffffffu, odd, d) || odd;
                 }
+                // sizes that a quotient of FP32 numbers can hold; smaller ones are zero in FP16 scores
+                worth[gr] = fmaxf(top, 1e-30f) / kDigits;
+                const float by = kDigits / fmaxf(top, 1e-30f);
+                int total = 0;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    uint32_t b[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int v = odd ? 0 : __float2int_rn(f[w][i] * by), hi = (v + 128) >> 8;
+                        total += v;
+                        b[i] = (uint32_t)(g & 1 ? v - hi * 256 : hi) & 0xff;
+                    }
+                    // bytes as the codes lie in a word: low nibbles 0, 2, 4, 6 are entries 0, 4, 1, 5, high ones 2, 6, 3, 7
+                    qd[n][gr][w][0] = b[0] | b[4] << 8 | b[1] << 16 | b[5] << 24;
+                    qd[n][gr][w][1] = b[2] | b[6] << 8 | b[3] << 16 | b[7] << 24;
+                }
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+                sum[gr] = (float)total;
+                if (odd) worth[gr] = NAN;                                  // a query that is not finite has no scores
             }
-            float sum[GR];
+            const int rt = St::row(n, t);
 #pragma unroll
             for (int gr = 0; gr < GR; gr++) {
-                sum[gr] = 0.f;
-#pragma unroll
-                for (int w = 0; w < 2; w++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const half2 h = __floats2half2_rn(f[gr][w][4 * j + 2 * i] * up, f[gr][w][4 * j + 2 * i + 1] * up);
-                            const float2 v = __half22float2(h);
-                            qf[n][gr][w][j][i] = bits(h);
-                            sum[gr] += v.x + v.y;
-                        }
-                sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
-                sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
+                qsum[n][gr] = __shfl_sync(0xffffffffu, sum[gr], 8 * t);
+                unit_q[n][gr] = __shfl_sync(0xffffffffu, worth[gr], 8 * t) * (a.scale * 1.4426950408889634f);
             }
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int src = 4 * (2 * t + i), rr = 8 * n + 2 * t + i;
-                col_scale[n][i] = __shfl_sync(0xffffffffu, down, src) * a.scale * 1.4426950408889634f;
-#pragma unroll
-                for (int gr = 0; gr < GR; gr++) qsum[n][i][gr] = __shfl_sync(0xffffffffu, sum[gr], src);
-                sees[n][i] = rr < tile_rows ? sp.position((r0 + rr) / per) + 1 : 0;
-                if (rr < tile_rows) least = min(least, sees[n][i]);
-            }
+            sees[n] = rt < tile_rows ? sp.position((r0 + rt) / per) + 1 : 0;
+            if (rt < tile_rows) least = min(least, sees[n]);
         }
         least = min(least, __shfl_xor_sync(0xffffffffu, least, 1));
         least = min(least, __shfl_xor_sync(0xffffffffu, least, 2));        // every row of the tile sees so many positions
 
-        float m[NT][2], l[NT][2], lo[NT][2][GR], o[NT][GR][4][4];
+        float m[NS], ref[NS], l[NS], lo[NS][GR], o[NC][GR][4][4];          // ref: m, 0 before the first position
         float largest = 0.f, unit = 0.f;                                   // power of two above every scale of values so far, kLift / it
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NS; n++) {
+            m[n] = -INFINITY;
+            ref[n] = l[n] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                m[n][i] = -INFINITY;
-                l[n][i] = 0.f;
+            for (int gr = 0; gr < GR; gr++) lo[n][gr] = 0.f;
+        }
 #pragma unroll
-                for (int gr = 0; gr < GR; gr++) lo[n][i][gr] = 0.f;
-            }
-#pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NC; n++)
 #pragma unroll
             for (int gr = 0; gr < GR; gr++)
 #pragma unroll
@@ -229,9 +251,7 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
         int slot = 0;
 #pragma unroll 1
         for (int j = j0 + warp; j < j1; j += kWarps) {
-            if (issued < j1) load(issued, slot == 0 ? St::kSlots - 1 : slot - 1);
-            issued += kWarps;
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            load(slot == 0 ? St::kSlots - 1 : slot - 1);
             asm volatile("cp.async.wait_group %0;" ::"n"(St::kSlots - 1) : "memory");
             __syncwarp();
             const uint8_t* kc = ring + slot * St::kSlot;
@@ -239,30 +259,33 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
             const int p0 = j * kStepChunk;
 
             // ---- scores ----
-            float s[NT][2][4];
+            float s[NS][2][2];                                             // set, half of the chunk, row g or g + 8 of the product
             bool grows = false;
-            float2 vpar[2][2][GR];                                         // (s, l) of values: product, upper or lower rows, group
+            float2 vpar[2][2][GR];                                         // (s, l + 8 s) of values
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 float2 par[2][GR];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const int row = 16 * h + 8 * u + place(g);
+                    uint32_t kw[GR], vw[GR];
+                    if constexpr (GR == 2) {
+                        const uint2 x2 = *reinterpret_cast<const uint2*>(kp + row * 8), y2 = *reinterpret_cast<const uint2*>(vp + row * 8);
+                        kw[0] = x2.x, kw[1] = x2.y, vw[0] = y2.x, vw[1] = y2.y;
+                    } else {
+                        kw[0] = *reinterpret_cast<const uint32_t*>(kp + row * 4), vw[0] = *reinterpret_cast<const uint32_t*>(vp + row * 4);
+                    }
 #pragma unroll
                     for (int gr = 0; gr < GR; gr++) {
-                        par[u][gr] = __half22float2(reinterpret_cast<const half2*>(kp)[row * GR + gr]);
-                        vpar[h][u][gr] = __half22float2(reinterpret_cast<const half2*>(vp)[row * GR + gr]);
+                        par[u][gr] = __half22float2(halves(kw[gr]));
+                        vpar[h][u][gr] = __half22float2(halves(vw[gr]));
                         vpar[h][u][gr].y = fmaf(8.f, vpar[h][u][gr].x, vpar[h][u][gr].y);
                         grows = grows || vpar[h][u][gr].x > largest;
                     }
                 }
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[n][h][e] = 0.f;
-#pragma unroll
                 for (int gr = 0; gr < GR; gr++) {
-                    float acc[NT][4] = {};
+                    int acc[NS][4] = {};
                     uint2 w[2];
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
@@ -271,33 +294,32 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                     }
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        uint32_t x[4], y[4];
-                        unpack8<0>(i ? w[0].y : w[0].x, x);
-                        unpack8<0>(i ? w[1].y : w[1].x, y);
+                        const uint32_t w0 = i ? w[0].y : w[0].x, w1 = i ? w[1].y : w[1].x;
+                        const uint32_t a0 = w0 & 0x0f0f0f0fu, a1 = w1 & 0x0f0f0f0fu, a2 = (w0 >> 4) & 0x0f0f0f0fu, a3 = (w1 >> 4) & 0x0f0f0f0fu;
 #pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            mma_f16(acc[n], x[0], y[0], x[1], y[1], qf[n][gr][i][0][0], qf[n][gr][i][0][1]);
-                            mma_f16(acc[n], x[2], y[2], x[3], y[3], qf[n][gr][i][1][0], qf[n][gr][i][1][1]);
-                        }
+                        for (int n = 0; n < NS; n++) mma_u8s8(acc[n], a0, a1, a2, a3, qd[n][gr][i][0], qd[n][gr][i][1]);
                     }
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+                    for (int n = 0; n < NS; n++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            s[n][h][e] = fmaf(par[e >> 1][gr].x, acc[n][e], fmaf(par[e >> 1][gr].y, qsum[n][e & 1][gr], s[n][h][e]));
+                        for (int u = 0; u < 2; u++) {
+                            const float dot = (float)(acc[n][2 * u] * 256 + acc[n][2 * u + 1]);
+                            const float v = fmaf(par[u][gr].x, dot, par[u][gr].y * qsum[n][gr]);
+                            s[n][h][u] = gr == 0 ? v * unit_q[n][gr] : fmaf(v, unit_q[n][gr], s[n][h][u]);
+                        }
                 }
             }
-            const bool masked = p0 + kStepChunk > least;
+            if (p0 + kStepChunk > least) {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+                for (int n = 0; n < NS; n++)
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                    for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        s[n][h][e] *= col_scale[n][e & 1];
-                        if (masked && p0 + 16 * h + 8 * (e >> 1) + place(g) >= sees[n][e & 1]) s[n][h][e] = -INFINITY;
-                        grows = grows || s[n][h][e] > m[n][e & 1] + kSlack;
-                    }
+                        for (int u = 0; u < 2; u++)
+                            if (p0 + 16 * h + 8 * u + place(g) >= sees[n]) s[n][h][u] = -INFINITY;
+            }
+#pragma unroll
+            for (int n = 0; n < NS; n++) grows = grows || fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][1][0], s[n][1][1])) > m[n] + kSlack;
             if (__any_sync(0xffffffffu, grows)) {
                 float top = largest;
 #pragma unroll
@@ -312,50 +334,58 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                 largest = top;
                 unit = top > 0.f ? kLift / top : 0.f;
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int n = 0; n < NS; n++) {
+                    float v = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][1][0], s[n][1][1]));
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        float x = fmaxf(fmaxf(s[n][0][i], s[n][0][2 + i]), fmaxf(s[n][1][i], s[n][1][2 + i]));
+                    for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+                    const float f = v > m[n] ? exp2_neg(m[n] - v) : 1.f;
+                    m[n] = fmaxf(m[n], v);
+                    ref[n] = m[n] == -INFINITY ? 0.f : m[n];
+                    l[n] *= f;
 #pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        const float f = x > m[n][i] ? exp2_neg(m[n][i] - x) : 1.f;
-                        m[n][i] = fmaxf(m[n][i], x);
-                        l[n][i] *= f;
+                    for (int gr = 0; gr < GR; gr++) {
+                        lo[n][gr] *= f;
 #pragma unroll
-                        for (int gr = 0; gr < GR; gr++) {
-                            lo[n][i][gr] *= f;
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                o[n][gr][k][i] *= f * shrink;
-                                o[n][gr][k][2 + i] *= f * shrink;
+                        for (int k = 0; k < 4; k++) {
+                            if constexpr (ROWS == 4) {
+                                o[0][gr][k][gr] *= f * shrink;
+                                o[0][gr][k][2 + gr] *= f * shrink;
+                            } else {
+                                o[n >> 1][gr][k][n & 1] *= f * shrink;
+                                o[n >> 1][gr][k][2 + (n & 1)] *= f * shrink;
                             }
                         }
                     }
+                }
             }
 
             // ---- weights, and outputs ----
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                uint32_t pw[NT][GR][2];
+                uint32_t pw[NC][GR][2];
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int u = 0; u < 2; u++) {
+                    float p[NS], f[GR];
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        float p[2];
+                    for (int gr = 0; gr < GR; gr++) f[gr] = vpar[h][u][gr].x * unit;
 #pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            p[i] = exp2_neg(s[n][h][2 * u + i] - (m[n][i] == -INFINITY ? 0.f : m[n][i]));
-                            l[n][i] += p[i];
-                        }
+                    for (int n = 0; n < NS; n++) {
+                        p[n] = exp2_neg(s[n][h][u] - ref[n]);
+                        l[n] += p[n];
 #pragma unroll
-                        for (int gr = 0; gr < GR; gr++) {
-                            const float2 par = vpar[h][u][gr];
-                            const float f = par.x * unit;
-                            lo[n][0][gr] = fmaf(p[0], par.y, lo[n][0][gr]);
-                            lo[n][1][gr] = fmaf(p[1], par.y, lo[n][1][gr]);
-                            pw[n][gr][u] = transposed(bits(__floats2half2_rn(p[0] * f, p[1] * f)));
-                        }
+                        for (int gr = 0; gr < GR; gr++) lo[n][gr] = fmaf(p[n], vpar[h][u][gr].y, lo[n][gr]);
                     }
+                    if constexpr (ROWS == 4) {
+                        pw[0][0][u] = transposed(bits(__floats2half2_rn(p[0] * f[0], GR == 2 ? p[0] * f[GR - 1] : 0.f)));
+#pragma unroll
+                        for (int gr = 1; gr < GR; gr++) pw[0][gr][u] = pw[0][0][u];
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < NC; n++)
+#pragma unroll
+                            for (int gr = 0; gr < GR; gr++) pw[n][gr][u] = transposed(bits(__floats2half2_rn(p[2 * n] * f[gr], p[2 * n + 1] * f[gr])));
+                    }
+                }
 #pragma unroll
                 for (int gr = 0; gr < GR; gr++) {
                     uint32_t w[4];                                         // positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the product
@@ -365,14 +395,14 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                         w[k] = *reinterpret_cast<const uint32_t*>(vc + row * (DIM / 2) + piece * 16 + (g & 3) * 4);
                     }
                     uint32_t x0[4], y0[4], x1[4], y1[4];                   // channels 8 g + 2 i and 8 g + 2 i + 1 of two positions each
-                    unpack8<8>(__byte_perm(w[0], w[1], 0x5410), x0);
-                    unpack8<8>(__byte_perm(w[0], w[1], 0x7632), y0);
-                    unpack8<8>(__byte_perm(w[2], w[3], 0x5410), x1);
-                    unpack8<8>(__byte_perm(w[2], w[3], 0x7632), y1);
+                    unpack8(__byte_perm(w[0], w[1], 0x5410), x0);
+                    unpack8(__byte_perm(w[0], w[1], 0x7632), y0);
+                    unpack8(__byte_perm(w[2], w[3], 0x5410), x1);
+                    unpack8(__byte_perm(w[2], w[3], 0x7632), y1);
 #pragma unroll
                     for (int i = 0; i < 4; i++)
 #pragma unroll
-                        for (int n = 0; n < NT; n++) mma_f16(o[n][gr][i], x0[i], y0[i], x1[i], y1[i], pw[n][gr][0], pw[n][gr][1]);
+                        for (int n = 0; n < NC; n++) mma_f16(o[n][gr][i], x0[i], y0[i], x1[i], y1[i], pw[n][gr][0], pw[n][gr][1]);
                 }
             }
             slot = slot + 1 == St::kSlots ? 0 : slot + 1;
@@ -382,47 +412,48 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
 
         // ---- the warps' parts of this head ----
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NS; n++) {
+            const int r = St::row(n, t);
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int r = 8 * n + 2 * t + i;
+            for (int d = 4; d < 32; d <<= 1) {
+                l[n] += __shfl_xor_sync(0xffffffffu, l[n], d);
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) {
-                    l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
-#pragma unroll
-                    for (int gr = 0; gr < GR; gr++) lo[n][i][gr] += __shfl_xor_sync(0xffffffffu, lo[n][i][gr], d);
-                }
-                if (g == 0) {
-                    stats[warp * 2 * St::kRows + r] = m[n][i];
-                    stats[(warp * 2 + 1) * St::kRows + r] = l[n][i];
-                }
-#pragma unroll
-                for (int gr = 0; gr < GR; gr++) {
-                    float* y = outs + warp * St::kOut + r * (DIM + kPad) + 64 * gr + 8 * g;
-                    const float back = largest / kLift;
-#pragma unroll
-                    for (int k = 0; k < 4; k += 2)
-                        *reinterpret_cast<float4*>(y + 2 * k) =
-                            make_float4(fmaf(o[n][gr][k][i], back, lo[n][i][gr]), fmaf(o[n][gr][k][2 + i], back, lo[n][i][gr]),
-                                        fmaf(o[n][gr][k + 1][i], back, lo[n][i][gr]), fmaf(o[n][gr][k + 1][2 + i], back, lo[n][i][gr]));
-                }
+                for (int gr = 0; gr < GR; gr++) lo[n][gr] += __shfl_xor_sync(0xffffffffu, lo[n][gr], d);
             }
+            if (g == 0) {
+                stats[warp * 2 * ROWS + r] = m[n];
+                stats[(warp * 2 + 1) * ROWS + r] = l[n];
+            }
+#pragma unroll
+            for (int gr = 0; gr < GR; gr++) {
+                float* y = outs + warp * St::kOut + r * (DIM + kPad) + 64 * gr + 8 * g;
+                const float back = largest / kLift;
+                const int nc = ROWS == 4 ? 0 : n >> 1, e = ROWS == 4 ? gr : n & 1;
+#pragma unroll
+                for (int k = 0; k < 4; k += 2)
+                    *reinterpret_cast<float4*>(y + 2 * k) =
+                        make_float4(fmaf(o[nc][gr][k][e], back, lo[n][gr]), fmaf(o[nc][gr][k][2 + e], back, lo[n][gr]),
+                                    fmaf(o[nc][gr][k + 1][e], back, lo[n][gr]), fmaf(o[nc][gr][k + 1][2 + e], back, lo[n][gr]));
+            }
+        }
         __syncthreads();
         const bool complete = j0 == 0 && j1 == chunks;
-        float* rec = complete ? nullptr : static_cast<float*>(a.ws) + ((size_t)blockIdx.x * 2 + (segment > 0)) * kRecord<DIM, St::kRows>;
+        float* rec = complete ? nullptr : record_of<DIM, ROWS>(a.ws, gridDim.x, blockIdx.x, segment > 0);
+        if (!complete && j0 == 0 && tid == 0)
+            *entry_of(a.ws, blockIdx.x) = Shared4{work.owner(x - 1, gridDim.x) - (int)blockIdx.x + 1, segment > 0, work.head, work.tile, sp.row0, sp.n, sp.len, 0};
         for (int e = tid; e < tile_rows * (DIM / 4); e += kThreads) {
             const int r = e / (DIM / 4), c = e % (DIM / 4) * 4;
             float top = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWarps; w++) top = fmaxf(top, stats[w * 2 * St::kRows + r]);
-            const float ref = top == -INFINITY ? 0.f : top;
+            for (int w = 0; w < kWarps; w++) top = fmaxf(top, stats[w * 2 * ROWS + r]);
+            const float zero = top == -INFINITY ? 0.f : top;
             float sum = 0.f;
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; w++) {
-                const float f = exp2_neg(stats[w * 2 * St::kRows + r] - ref);
+                const float f = exp2_neg(stats[w * 2 * ROWS + r] - zero);
                 const float4 v = *reinterpret_cast<const float4*>(outs + w * St::kOut + r * (DIM + kPad) + c);
-                sum = fmaf(stats[(w * 2 + 1) * St::kRows + r], f, sum);
+                sum = fmaf(stats[(w * 2 + 1) * ROWS + r], f, sum);
                 y = make_float4(fmaf(v.x, f, y.x), fmaf(v.y, f, y.y), fmaf(v.z, f, y.z), fmaf(v.w, f, y.w));
             }
             if (complete) {
@@ -431,58 +462,58 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
             } else {
                 if (c == 0) {
                     rec[r] = top;
-                    rec[St::kRows + r] = sum;
+                    rec[ROWS + r] = sum;
                 }
-                *reinterpret_cast<float4*>(rec + 2 * St::kRows + r * DIM + c) = y;
+                *reinterpret_cast<float4*>(rec + 2 * ROWS + r * DIM + c) = y;
             }
         }
         __syncthreads();
-        x += whole ? 1 : j1 - j0;
         if (x < to) work.next();
     }
 }
 
-template <typename T, int DIM, int NT>
+template <typename T, int DIM, int ROWS>
 int launch(const Cache4Call& a, Rows<const T> q, Rows<T> out, const StepPlan& p, cudaStream_t stream)
 {
-    using St = Step<DIM, NT>;
     static bool attr[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return fail(TLLM_ERR_LAUNCH, "cache4_step: no current device");
     if (!attr[dev]) {
-        cudaFuncSetAttribute(cache4_step_kernel<T, DIM, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, St::kSmem);
+        cudaFuncSetAttribute(cache4_step_kernel<T, DIM, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Step<DIM, ROWS>::kSmem);
         attr[dev] = true;
     }
-    int st = launch_pdl("cache4_step", cache4_step_kernel<T, DIM, NT>, dim3(p.ctas), dim3(kThreads), St::kSmem, stream, a, q, out, p.whole);
+    int st = launch_pdl("cache4_step", cache4_step_kernel<T, DIM, ROWS>, dim3(p.ctas), dim3(kThreads), Step<DIM, ROWS>::kSmem, stream, a, q, out, p.whole);
     if (st || p.whole) return st;
-    return launch_cache4_join<T>(a, out, St::kRows, p.ctas, p.items, stream);
+    return launch_cache4_join<T>(a, out, ROWS, p.ctas, stream);
+}
+
+template <typename T, int DIM>
+int launch_rows(const Cache4Call& a, Rows<const T> q, Rows<T> out, const StepPlan& p, cudaStream_t stream)
+{
+    return p.rows == 4 ? launch<T, DIM, 4>(a, q, out, p, stream) : p.rows == 8 ? launch<T, DIM, 8>(a, q, out, p, stream) : launch<T, DIM, 16>(a, q, out, p, stream);
 }
 
 }  // namespace
 
-// Rows of a tile: 8, or 16 where that saves a walk over the cache.
 StepPlan step_plan(const Cache4& c, int tokens, int heads, int max_new, int max_len)
 {
     StepPlan p;
-    const int per = heads / c.kv_heads, most = max_new > 0 ? max_new : (tokens + c.batch - 1) / (c.batch > 0 ? c.batch : 1);
+    const int per = heads / c.kv_heads, most = max_new > 0 && max_new < tokens ? max_new : (tokens + c.batch - 1) / c.batch;
     const long long rows = (long long)most * per;
-    p.tiles = rows > 8 ? 2 : 1;
-    const long long items = (long long)c.batch * c.kv_heads * ((rows + 8 * p.tiles - 1) / (8 * p.tiles));
-    p.items = (int)(items < 1 ? 1 : items < 65536 ? items : 65536);
+    p.rows = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    const long long items = (long long)c.batch * c.kv_heads * ((rows + p.rows - 1) / p.rows);
     const int len = max_len > 0 && max_len < c.rows ? max_len : c.rows;
-    const int at_once = p.tiles == 1 ? 296 : 148;
     p.whole = len <= 512;
-    p.ctas = p.whole ? p.items : at_once;
-    p.bytes = p.whole ? 0 : (size_t)p.ctas * 2 * (size_t)(8 * p.tiles) * (c.dim + 2) * sizeof(float);
+    p.ctas = p.whole ? (int)(items < 65536 ? items : 65536) : p.rows == 16 ? 148 : 296;
+    p.bytes = p.whole ? 0 : join_bytes(c.dim, p.rows, p.ctas);
     return p;
 }
 
 template <typename T>
 int launch_cache4_step(const Cache4Call& a, Rows<const T> q, Rows<T> out, const StepPlan& p, cudaStream_t stream)
 {
-    if (a.c.dim == 64) return p.tiles == 1 ? launch<T, 64, 1>(a, q, out, p, stream) : launch<T, 64, 2>(a, q, out, p, stream);
-    return p.tiles == 1 ? launch<T, 128, 1>(a, q, out, p, stream) : launch<T, 128, 2>(a, q, out, p, stream);
+    return a.c.dim == 64 ? launch_rows<T, 64>(a, q, out, p, stream) : launch_rows<T, 128>(a, q, out, p, stream);
 }
 
 template int launch_cache4_step<half>(const Cache4Call&, Rows<const half>, Rows<half>, const StepPlan&, cudaStream_t);

@@ -1,5 +1,6 @@
 // The work of a call over the 4-bit cache as one sequence of units, computed on the device from the
-// sequences' lengths: tiles of rows of key/value heads, each a number of chunks of positions.
+// sequences' lengths: tiles of rows of key/value heads, each a number of chunks of positions and what a tile costs
+// beside them.
 #pragma once
 #include "cache4.cuh"
 
@@ -10,10 +11,26 @@ constexpr int kPromptChunk = 128, kPromptRows = 256; // positions and rows a CTA
 // Floats of the part of a tile's rows that one CTA found: maxima, sums, outputs.
 template <int DIM, int ROWS> constexpr int kRecord = ROWS * (DIM + 2);
 
+// A tile of rows that several CTAs share, written by the one that has its first chunk (parts = 0 by a CTA that has none): its
+// record is its first or second one, those of the CTAs behind it are their first.
+struct Shared4 {
+    int parts, slot, head, tile, row0, n, len, unused;
+};
+// Workspace: an entry of each CTA, then two records of each.
+inline size_t join_bytes(int dim, int rows, int ctas) { return (size_t)ctas * (sizeof(Shared4) + 2 * (size_t)rows * (dim + 2) * sizeof(float)); }
+#ifdef __CUDACC__
+__device__ __forceinline__ Shared4* entry_of(void* ws, int cta) { return static_cast<Shared4*>(ws) + cta; }
+template <int DIM, int ROWS>
+__device__ __forceinline__ float* record_of(void* ws, int ctas, int cta, int slot)
+{
+    return reinterpret_cast<float*>(static_cast<Shared4*>(ws) + ctas) + ((size_t)cta * 2 + slot) * kRecord<DIM, ROWS>;
+}
+#endif
+
 struct StepPlan {
-    int tiles;                                       // of 8 rows that go through the cache together
+    int rows;                                        // that go through the cache together: 4, 8 or 16
     bool whole;                                      // a tile's positions stay in one CTA
-    int ctas, items;
+    int ctas;
     size_t bytes;
 };
 StepPlan step_plan(const Cache4& c, int tokens, int heads, int max_new, int max_len);
@@ -22,23 +39,26 @@ int launch_cache4_step(const Cache4Call& a, Rows<const T> q, Rows<T> out, const 
 
 struct PromptPlan {
     bool whole;
-    int ctas, items;
-    size_t bytes;
+    int ctas, cap;                                   // cap: positions of a sequence that are expanded first, 0: none
+    size_t join_bytes, bytes;
 };
 PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int max_len);
 template <typename T>
 int launch_cache4_prompt(const Cache4Call& a, Rows<const T> q, Rows<T> out, const PromptPlan& p, cudaStream_t stream);
 
-// Joins what several of `ctas` CTAs found for one tile of rows; items: about how many tiles there are (cache4_join.cu).
+// Joins what several of `ctas` CTAs found for one tile of rows (cache4_join.cu).
 template <typename T>
-int launch_cache4_join(const Cache4Call& a, Rows<T> out, int rows, int ctas, int items, cudaStream_t stream);
+int launch_cache4_join(const Cache4Call& a, Rows<T> out, int rows, int ctas, cudaStream_t stream);
 
 #ifdef __CUDACC__
 // Row r of sequence b and key/value head `head` is query head r % per of the head's, of new token r / per; a tile is R of
-// them.  Units are chunks of positions, or whole tiles.  Members are found by whole warps, every lane with the same result.
+// them.  Units are whole tiles, or chunks of positions behind kFixed units a tile (its rows' loading, joining and
+// storing, in chunks), so that CTAs with many short tiles and CTAs with a part of a long one take equally long.  Members are
+// found by whole warps, every lane with the same result.
 template <int R, int CHUNK>
 struct Work {
-    static constexpr int kLeast = CHUNK == kStepChunk ? 16 : 2;            // chunks that a CTA takes at least where work is cut
+    static constexpr int kFixed = CHUNK == kStepChunk ? 8 : 2;
+    static constexpr int kLeast = CHUNK == kStepChunk ? 24 : 4;            // units that a CTA takes at least where work is cut
     Seqs s;
     int per, kv_heads;
     bool whole;
@@ -53,20 +73,57 @@ struct Work {
         return max(sp.position(last / per) + 1, 0);
     }
     __device__ __forceinline__ int chunks_of(const Span& sp, int tl) const { return max((seen(sp, tl) + CHUNK - 1) / CHUNK, 1); }
-    // units of a head of a sequence
-    __device__ __forceinline__ long long units(const Span& sp) const
+    __device__ __forceinline__ int units_of(const Span& sp, int tl) const { return kFixed + chunks_of(sp, tl); }
+    // the first chunk at or behind unit u of a tile, and the unit where it begins
+    static __device__ __forceinline__ int chunk_at(long long u) { return u > kFixed ? (int)u - kFixed : 0; }
+    __device__ __forceinline__ int tiles_of(const Span& sp) const { return (int)(((long long)sp.n * per + R - 1) / R); }
+    // units of a head of each lane's sequence; the lanes share the tiles of one where there are many
+    __device__ __forceinline__ long long units(const Span& sp, int lane) const
     {
-        const int tiles = (int)(((long long)sp.n * per + R - 1) / R);
+        const int tiles = tiles_of(sp);
         if (whole) return tiles;
         long long sum = 0;
-        for (int i = 0; i < tiles; i++) sum += chunks_of(sp, i);
+        if (__all_sync(0xffffffffu, tiles <= 2)) {
+            for (int i = 0; i < tiles; i++) sum += units_of(sp, i);
+            return sum;
+        }
+        for (uint32_t left = __ballot_sync(0xffffffffu, tiles > 0); left; left &= left - 1) {
+            const int from = __ffs(left) - 1, n = __shfl_sync(0xffffffffu, tiles, from);
+            Span one;
+            one.n = __shfl_sync(0xffffffffu, sp.n, from);
+            one.len = __shfl_sync(0xffffffffu, sp.len, from);
+            long long part = 0;
+            for (int i = lane; i < n; i += 32) part += units_of(one, i);
+            part = warp_total(part);
+            if (lane == from) sum = part;
+        }
         return sum;
+    }
+    static __device__ __forceinline__ long long warp_total(long long v)
+    {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+    static __device__ __forceinline__ long long warp_scan(long long v, int lane)
+    {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long w = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += w;
+        }
+        return v;
+    }
+    __device__ __forceinline__ Span lane_span(int i) const
+    {
+        Span none;
+        none.row0 = none.n = none.len = 0;
+        return i < s.batch ? span_of(s, i, false) : none;
     }
     __device__ __forceinline__ Work(const Seqs& s_, int per_, int kv_heads_, bool whole_, int lane) : s(s_), per(per_), kv_heads(kv_heads_), whole(whole_), total(0)
     {
-        for (int i = lane; i < s.batch; i += 32) total += units(span_of(s, i, false)) * kv_heads;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        for (int b0 = 0; b0 < s.batch; b0 += 32) total += units(lane_span(b0 + lane), lane) * kv_heads;
+        total = warp_total(total);
     }
     // first unit of part c of `parts`
     __device__ __forceinline__ int used(int parts) const
@@ -88,45 +145,40 @@ struct Work {
         visible = seen(span, tl);
         chunks = max((visible + CHUNK - 1) / CHUNK, 1);
     }
-    // units of all sequences before b
-    __device__ __forceinline__ long long before(int seq, int lane) const
-    {
-        long long sum = 0;
-        for (int i = lane; i < seq; i += 32) sum += units(span_of(s, i, false)) * kv_heads;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        return sum;
-    }
     // unit x < total
     __device__ __forceinline__ void find(long long x, int lane)
     {
+        long long u = 0;                              // of a head of the sequence
         for (int b0 = 0; b0 < s.batch; b0 += 32) {
-            long long mine = b0 + lane < s.batch ? units(span_of(s, b0 + lane, false)) * kv_heads : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, mine, o);
-                if (lane >= o) mine += v;
-            }
-            const uint32_t m = __ballot_sync(0xffffffffu, mine > x);
+            const long long mine = units(lane_span(b0 + lane), lane), up_to = warp_scan(mine * kv_heads, lane);
+            const uint32_t m = __ballot_sync(0xffffffffu, up_to > x);
             const int at = m ? __ffs(m) - 1 : 31;
-            const long long below = __shfl_sync(0xffffffffu, mine, at > 0 ? at - 1 : 0);
-            if (m) {
-                b = b0 + at;
-                x -= at > 0 ? below : 0;
-                break;
-            }
-            x -= __shfl_sync(0xffffffffu, mine, 31);
+            u = __shfl_sync(0xffffffffu, mine, at);
+            const long long end = __shfl_sync(0xffffffffu, up_to, at);
+            x -= m ? end - u * kv_heads : end;
+            b = b0 + at;
+            if (m) break;
         }
         span = span_of(s, b, false);
         rows = span.n * per;
-        const long long u = units(span);
         head = (int)(x / u);
         x -= head * u;
         int tl = 0;
         offset = 0;
         if (whole) tl = (int)x;
         else {
-            for (int n; x >= (n = chunks_of(span, tl)); tl++) x -= n;
+            const int tiles = tiles_of(span);
+            for (;; tl += 32) {
+                const long long mine = tl + lane < tiles ? units_of(span, tl + lane) : 0, up_to = warp_scan(mine, lane);
+                const uint32_t m = __ballot_sync(0xffffffffu, up_to > x);
+                const int at = m ? __ffs(m) - 1 : 31;
+                const long long end = __shfl_sync(0xffffffffu, up_to, at);
+                x -= m ? end - __shfl_sync(0xffffffffu, mine, at) : end;
+                if (m) {
+                    tl += at;
+                    break;
+                }
+            }
             offset = (int)x;
         }
         set_tile(tl);

@@ -213,6 +213,21 @@ def test_padding_and_sequences_outside_the_tensors():
             tl.check_device_errors()
 
 
+@pytest.mark.parametrize("new", [1, 9, 300])
+def test_sequences_above_the_limit_of_a_call(new):
+    c = new_cache(1, 2, 1200, 64)
+    x = torch.randn(1000, 2, 64, device="cuda").half()
+    ops.append(c, None, x, x, ints(0, 1000), ints(1000))
+    q, out = torch.randn(new, 4, 64, device="cuda").half(), torch.empty(new, 4, 64, device="cuda", dtype=torch.float16)
+    ops.attention(c, q, out, ints(0, new), ints(1000), max_new=new, max_len=1000)
+    tl.check_device_errors()
+    check_attention(c, q, out, [1000 - new], [new], 4, torch.float16, 0.125)
+    ops.attention(c, q, out, ints(0, new), ints(1000), max_new=new, max_len=900)
+    with pytest.raises(tl.TllmError, match="outside its tensors"):
+        tl.check_device_errors()
+    check_attention(c, q, out, [900 - new], [new], 4, torch.float16, 0.125)          # as a sequence of 900 positions
+
+
 def test_nothing_to_do():
     for batch, tokens in ((0, 0), (2, 0), (0, 3)):
         c = ops.Cache4.empty(batch, 2, 8, 64)
@@ -304,9 +319,9 @@ def test_prompts(dtype, before, new, heads, kv_heads, dim):
 
 
 @pytest.mark.parametrize("new", [[1, 1], [3, 40], [200, 130]])
-@pytest.mark.parametrize("new_hint,len_hint", [(0, 0), (1, 1), (5, 100), (1000, 100000)])
+@pytest.mark.parametrize("new_hint,len_hint", [(0, 0), (1, 2700), (5, 0), (1000, 100000), (90, 2700), (1, 0)])
 def test_hints_do_not_matter(new, new_hint, len_hint):
-    """Wrong hints choose another way of the work, not another result."""
+    """Wrong numbers of rows choose another way of the work, not another result; so do loose limits of positions."""
     gen = torch.Generator(device="cuda").manual_seed(5)
     before, lens = [400, 2500], [400 + new[0], 2500 + new[1]]
     c = random_cache(gen, 2, 2, 3000, 128, lens)
