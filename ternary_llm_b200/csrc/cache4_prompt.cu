@@ -1,9 +1,8 @@
 // Attention over the 4-bit key/value cache for many rows a sequence, on the 5th-generation tensor cores.
 //
 // A CTA takes 256 rows of a key/value head (new tokens times the query heads that share it) as two tiles of 128 and
-// walks over tiles of 128 positions.  Roles: four warps turn the codes of keys into FP16 numbers in shared memory,
-// rounded once (l + s c, 11 bits), three those of values; one issues tcgen05.mma; four for each tile of rows have a row
-// a thread.
+// walks over tiles of 128 positions.  Roles: six warps turn codes into FP16 numbers in shared memory, rounded once
+// (l + s c, 11 bits); one for each tile of rows issues tcgen05.mma; four for each tile of rows have a row a thread.
 //   S = Q K^T    both operands in shared memory, 128 FP32 columns of tensor memory for each tile of rows
 //   softmax      a thread reads its row; the weights go back over S as FP16, with a factor of 2^6 that leaves small
 //                ones their bits (the sum of the weights takes it out)
@@ -32,22 +31,19 @@ namespace {
 using namespace gemm;
 
 constexpr int kTile = kPromptChunk, kRows = kPromptRows, kRowTiles = kRows / kTile;
-constexpr int kThreads = 512;                        // warps: rows' softmax 0-3 and 4-7, keys 8-11, products 12, values 13-15
-constexpr int kValueThreads = 96;
-// registers of a softmax thread, of the others: 2 * many + 2 * few = 4 * 128
-template <bool UNPACK> constexpr int kMany = UNPACK ? 184 : 200;
-template <bool UNPACK> constexpr int kFew = 256 - kMany<UNPACK>;
+constexpr int kThreads = 512;                        // warps: softmax of a tile of rows 0-3, of the other 4-7, its products 12, 13, keys and values the rest
+constexpr int kUnpackThreads = 192;
 constexpr int kBlock = kTile * 128;                  // bytes of 64 columns of a tile: 128-byte rows
-constexpr int kStages = 2;
+constexpr int kStages = 2, kHalf = kTile / 2;
 constexpr float kSlack = 8.f, kLift = 6.f, kLog2e = 1.4426950408889634f;
 
 template <int DIM>
 struct Prompt {
     static constexpr int kBlocks = DIM / 64;
     static constexpr int kOperand = kBlocks * kBlock;                              // bytes of a tile
-    static constexpr int kValueRounds = (DIM / 32 * kTile + kValueThreads - 1) / kValueThreads;
-    static constexpr int kRawKeys = kTile * (DIM / 2 + 4 * kBlocks), kRaw = kRawKeys + kValueRounds * kValueThreads * 20;     // the next tile's codes and params
-    static constexpr int kSmem = (kRowTiles + 2 * kStages) * kOperand + kRaw + 1024;
+    static constexpr int kRounds = (DIM / 32 * kTile + kUnpackThreads - 1) / kUnpackThreads;      // of 16 bytes a thread, of keys or values
+    static constexpr int kRawSide = kRounds * kUnpackThreads * 20;                                // the next tile's codes and params
+    static constexpr int kSmem = (kRowTiles + 2 * kStages) * kOperand + 2 * kRawSide + 1024;
     static constexpr uint32_t kTmemCols = kRowTiles * (kTile + DIM) <= 384 && kRowTiles * (kTile + DIM) > 256 ? 512 : kRowTiles * (kTile + DIM);
 };
 
@@ -89,7 +85,6 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool v
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid ? N : 0) : "memory");
 }
-__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -117,13 +112,12 @@ __device__ __forceinline__ f32x2 fma_pairs(f32x2 a, f32x2 b, f32x2 c)
     fma_pair(c, a, b);
     return c;
 }
+__device__ __forceinline__ f32x2 neg_pair(f32x2 v) { return v ^ 0x8000000080000000ull; }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // Keys and values as FP16 rows: [batch * kv_heads][cap][dim].
 struct Expanded {
@@ -134,23 +128,19 @@ struct Expanded {
 // A tile's rows of a key/value head and the tiles of positions [j0, j1) of its `chunks`, one after the other for this CTA;
 // every role walks over the same.
 struct Walk : Work<kRows, kTile> {
-    long long x, to;
     int from_top, step, j0, j1, segment;
-    __device__ __forceinline__ Walk(const Cache4Call& a, bool whole_, int lane) : Work(a.s, a.heads / a.c.kv_heads, a.c.kv_heads, whole_, lane), segment(-1)
+    __device__ __forceinline__ Walk(const Cache4Call& a, bool whole_, const Start& f) : Work(a.s, a.heads / a.c.kv_heads, a.c.kv_heads, whole_), segment(-1)
     {
         if (whole) {
-            const int pairs = s.batch * kv_heads;
-            from_top = (int)(blockIdx.x / pairs);
+            const int pairs = s.batch * kv_heads, pair = blockIdx.x % pairs;
             step = max((int)gridDim.x / pairs, 1);
-            b = (int)(blockIdx.x % pairs) / kv_heads;
-            head = (int)(blockIdx.x % pairs) % kv_heads;
-            span = span_of(s, b, false);
+            from_top = (int)blockIdx.x / pairs - step;
+            b = pair / kv_heads;
+            head = pair % kv_heads;
+            span = span_of(s, b, blockIdx.x / pairs == 0 && head == 0 && threadIdx.x == 0);
             rows = span.n * per;
-            from_top -= step;
         } else {
-            x = start(blockIdx.x, gridDim.x);
-            to = start(blockIdx.x + 1, gridDim.x);
-            if (x < to) find(x, lane);
+            begin(f);
         }
     }
     __device__ __forceinline__ bool advance()
@@ -169,7 +159,7 @@ struct Walk : Work<kRows, kTile> {
             if (x >= to) return false;
             if (++segment > 0) next();
             j0 = chunk_at(offset);
-            j1 = chunk_at(min((long long)kFixed + chunks, offset + (to - x)));
+            j1 = chunk_at(min(kFixed + chunks, offset + (to - x)));
             x += kFixed + chunks - offset;
         } while (j0 == j1);
         return true;
@@ -178,13 +168,32 @@ struct Walk : Work<kRows, kTile> {
     __device__ __forceinline__ int tile_rows(int i) const { return min(kTile, rows - tile * kRows - i * kTile); }
 };
 
-enum Bar { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPvDone = 12, kPReady = 14, kLast = 18, kBars = 19 };
+// the last three by tile of rows and half of a tile of positions
+enum Bar { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPvDone = 14, kPReady = 18, kLast = 22, kBars = 24 };
 
+// the largest; NaN where one of them is
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+// Of every kEvery pairs of weights kPolynomial come from multiplications and additions, the others from the unit of special
+// functions, which takes a warp's instruction every eight clocks and would be the limit.
+constexpr int kEvery = 4, kPolynomial = 0;
+// 2^x of two numbers: x = n + f with n = rint(x) in the low bits of x + 1.5 * 2^23, a polynomial in f (|f| <= 1/2, of degree 4 with the
+// smallest largest relative error, 2.6e-6), and n added to the exponent.  Below -126: 2^-126.  A NaN gives any number.
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 v)
+{
+    float2 x = split_f32(v);
+    v = pair_f32(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+    const f32x2 magic = pair_f32(12582912.f, 12582912.f), t = add_pair(v, magic), f = add_pair(v, neg_pair(add_pair(t, neg_pair(magic))));
+    f32x2 p = fma_pairs(f, pair_f32(0.009570102207362652f, 0.009570102207362652f), pair_f32(0.05591785907745361f, 0.05591785907745361f));
+    p = fma_pairs(p, f, pair_f32(0.240247443318367f, 0.240247443318367f));
+    p = fma_pairs(p, f, pair_f32(0.6931217908859253f, 0.6931217908859253f));
+    p = fma_pairs(p, f, pair_f32(0.9999992847442627f, 0.9999992847442627f));
+    const float2 n = split_f32(t), y = split_f32(p);
+    return pair_f32(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23), __float_as_uint(y.y) + (__float_as_uint(n.y) << 23));
 }
 // 32 codes as l + s c, rounded to FP16.
 __device__ __forceinline__ void expand32(const uint4& code, half2 par, uint4 (&y)[4])
@@ -228,6 +237,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
     __shared__ __align__(8) uint64_t bars[kBars];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
+    __shared__ Walk::Start start;
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t *qs = smem, *ks = qs + kRowTiles * P::kOperand, *vs = ks + kStages * P::kOperand, *raw = vs + kStages * P::kOperand;
@@ -239,7 +249,8 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
     if (tid == 0) {
         for (int i = 0; i < kBars; i++) {
             const int pair = i & ~1;
-            mbar_init(bar(i), pair == kQFull || (UNPACK && pair == kKFull) || (i >= kPReady && i < kLast) ? kTile : UNPACK && pair == kVFull ? kValueThreads : 1);
+            mbar_init(bar(i), pair == kQFull || (i >= kPReady && i < kLast) ? kTile : UNPACK && (pair == kKFull || pair == kVFull) ? kUnpackThreads :
+                              pair == kKEmpty || pair == kVEmpty ? kRowTiles : 1);
         }
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -249,215 +260,178 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(P::kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    pdl_wait();
+    if (warp == 13 && !whole) Walk::Work(a.s, a.heads / a.c.kv_heads, a.c.kv_heads, false).find(blockIdx.x, gridDim.x, lane, &start);
+    if (!whole && tid == 0) entry_of(a.ws, blockIdx.x)->parts = 0;
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot;                                       // S of both tiles of rows, then O of both
-    pdl_wait();
-    if (blockIdx.x == 0 && warp == 13)
-        for (int b = lane; b < a.s.batch; b += 32) span_of(a.s, b, true);
 
-    if (warp >= 12) {
-        fewer_registers<kFew<UNPACK>>();
-        if (warp == 12) {
-            // ---------------- products ----------------
-            // Every value that a branch or an operand depends on is uniform by a vote or a reduction of the warp: operands then come from
-            // uniform registers (some 150 clocks an MMA otherwise).
-            const bool leader = elect_one();
-            const uint32_t id_s = idesc(kTile, false), id_o = idesc(DIM, true), base = uniform(smem_u32(smem)), t0 = uniform(tmem);
-            const auto wait = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar(i), parity, abortp)) != 0; };
-            const auto score = [&](int i, uint32_t st) {
-                const uint64_t qd = make_sw128_desc(base + i * P::kOperand), kd = make_sw128_desc(base + (kRowTiles + st) * P::kOperand);
+    if (warp == 12 || warp == 13) {
+        // ---------------- products of a tile of rows ----------------
+        // Every value that a branch or an operand depends on is uniform by a vote or a reduction of the warp: operands then come from
+        // uniform registers (some 150 clocks an MMA otherwise).
+        const int i = warp - 12;
+        const bool leader = elect_one();
+        const uint32_t id_s = idesc(kHalf, false), id_o = idesc(DIM, true), t0 = uniform(tmem), base = uniform(smem_u32(smem));
+        const uint64_t qd = make_sw128_desc(base + i * P::kOperand);
+        const uint32_t to_s = t0 + i * kTile, to_o = t0 + kRowTiles * kTile + i * DIM;
+        const auto wait = [&](int k, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar(k), parity, abortp)) != 0; };
+        // half h of a tile of positions
+        const auto score = [&](int h, uint32_t st) {
+            const uint64_t kd = make_sw128_desc(base + (kRowTiles + st) * P::kOperand) + h * (kHalf * 128 >> 4);
+            fence_after();
 #pragma unroll
-                for (int j = 0; j < P::kBlocks; j++)
+            for (int j = 0; j < P::kBlocks; j++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t o = j * (kBlock >> 4) + k * 2;
-                        mma_ss(leader, t0 + i * kTile, qd + o, kd + o, id_s, j > 0 || k > 0);
-                    }
-                commit(leader, bar(kSFull + i));
-            };
-            // half of the positions of a tile
-            const auto output = [&](int i, uint32_t st, int part, bool first) {
-                const uint64_t vd = feature_major_desc(base + (kRowTiles + kStages + st) * P::kOperand);
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t o = j * (kBlock >> 4) + k * 2;
+                    mma_ss(leader, to_s + h * kHalf, qd + o, kd + o, id_s, j > 0 || k > 0);
+                }
+            commit(leader, bar(kSFull + i + 2 * h));
+        };
+        const auto output = [&](int h, uint32_t st, bool first) {
+            const uint64_t vd = feature_major_desc(base + (kRowTiles + kStages + st) * P::kOperand) + h * (kHalf * 128 >> 4);
+            fence_after();
 #pragma unroll
-                for (int k = part * 4; k < part * 4 + 4; k++)
-                    mma_ts(leader, t0 + kRowTiles * kTile + i * DIM, t0 + i * kTile + k * 8, vd + k * (2048 >> 4), id_o, !first || k > 0);
-                if (part) commit(leader, bar(kPvDone + i));
-            };
-            Walk w(a, whole, lane);
-            uint32_t n = 0, items[2] = {0, 0}, rounds[2] = {0, 0};         // tiles of positions so far; by tile of rows: segments, weights
-            bool ok = true;
-            while (ok && __any_sync(0xffffffffu, w.advance())) {
-                const int active = uniform(w.tile_rows(1) > 0 ? 2 : 1), tiles = uniform(w.j1 - w.j0);
-                ok = wait(kKFull + (n & 1), (n >> 1) & 1);
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-                    if (ok && i < active) {
-                        ok = wait(kQFull + i, items[i]++ & 1);
-                        fence_after();
-                        if (ok) score(i, n & 1);
-                    }
-                if (ok) commit(leader, bar(kKEmpty + (n & 1)));
+            for (int k = 0; k < kHalf / 16; k++) mma_ts(leader, to_o, to_s + h * kHalf + k * 8, vd + k * (2048 >> 4), id_o, !first || k > 0);
+            commit(leader, bar(kPvDone + i + 2 * h));
+        };
+        Walk w(a, whole, start);
+        uint32_t n = 0, items = 0, rounds = 0;                             // tiles of positions so far; with rows here: segments, tiles
+        bool ok = true;
+        while (ok && __any_sync(0xffffffffu, w.advance())) {
+            const int tiles = uniform(w.j1 - w.j0);
+            if (!uniform(w.tile_rows(i) > 0)) {
+                // no rows here: the stages are free as soon as they are full
                 for (int j = 0; ok && j < tiles; j++, n++) {
-                    const uint32_t st = n & 1;
-                    const bool more = j + 1 < tiles;
-                    ok = wait(kVFull + st, (n >> 1) & 1);
+                    ok = wait(kKFull + (n & 1), (n >> 1) & 1) && wait(kVFull + (n & 1), (n >> 1) & 1);
+                    if (ok && lane == 0) {
+                        mbar_arrive(bar(kKEmpty + (n & 1)));
+                        mbar_arrive(bar(kVEmpty + (n & 1)));
+                    }
+                }
+                continue;
+            }
+            ok = wait(kKFull + (n & 1), (n >> 1) & 1) && wait(kQFull + i, items++ & 1);
+            if (ok) {
+                score(0, n & 1);
+                score(1, n & 1);
+                commit(leader, bar(kKEmpty + (n & 1)));
+            }
+            for (int j = 0; ok && j < tiles; j++, n++, rounds++) {
+                const uint32_t st = n & 1, parity = rounds & 1;
+                ok = wait(kVFull + st, (n >> 1) & 1);
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        if (i < active) {
-#pragma unroll
-                            for (int part = 0; part < 2; part++) {
-                                ok = ok && wait(kPReady + 2 * i + part, rounds[i] & 1);
-                                if (!ok) break;
-                                fence_after();
-                                output(i, st, part, j == 0);
-                            }
-                            if (ok && more) {
-                                // the weights lie where the next scores go
-                                ok = (i > 0 || wait(kKFull + (st ^ 1), ((n + 1) >> 1) & 1)) && wait(kPvDone + i, rounds[i] & 1);
-                                fence_after();
-                                if (ok) score(i, st ^ 1);
-                            }
-                            rounds[i]++;
-                        }
-                    if (ok) {
-                        commit(leader, bar(kVEmpty + st));
-                        if (more) commit(leader, bar(kKEmpty + (st ^ 1)));
+                for (int h = 0; h < 2; h++) {
+                    ok = ok && wait(kPReady + i + 2 * h, parity);
+                    if (!ok) break;
+                    output(h, st, j == 0 && h == 0);
+                    if (h == 1) commit(leader, bar(kVEmpty + st));
+                    if (j + 1 < tiles) {
+                        // the weights lie where the next scores go
+                        ok = (h > 0 || wait(kKFull + (st ^ 1), ((n + 1) >> 1) & 1)) && wait(kPvDone + i + 2 * h, parity);
+                        if (!ok) break;
+                        score(h, st ^ 1);
+                        if (h == 1) commit(leader, bar(kKEmpty + (st ^ 1)));
                     }
                 }
             }
-            if (!ok) {
-                abort_flag = 1;
-                // what was issued completes before the memory is given up
-                commit(leader, bar(kLast));
-                __syncwarp();
-                mbar_wait(bar(kLast), 0, &never);
-            }
-        } else if constexpr (!UNPACK) {
-            if (warp == 13) {
-                // ---------------- copies of expanded keys and values ----------------
-                const bool leader = elect_one();
-                Walk w(a, whole, lane);
-                uint32_t n = 0, issued[2] = {0, 0};
-                bool ok = true;
-                while (ok && w.advance()) {
-                    const int row0 = (w.b * w.kv_heads + w.head) * x.cap;
-                    for (int j = w.j0; ok && j < w.j1; j++, n++) {
-                        const uint32_t st = n & 1, parity = ((n >> 1) & 1) ^ 1;
-#pragma unroll
-                        for (int side = 0; side < 2; side++) {
-                            const uint32_t full = bar((side ? kVFull : kKFull) + st);
-                            if (!(ok = mbar_wait(bar((side ? kVEmpty : kKEmpty) + st), parity, abortp))) break;
-                            if (leader) {
-                                mbar_expect_tx(full, P::kOperand);
-#pragma unroll
-                                for (int c = 0; c < P::kBlocks; c++)
-                                    tma_load_2d(smem_u32((side ? vs : ks) + st * P::kOperand + c * kBlock), side ? &x.v : &x.k, c * 64, row0 + j * kTile, full);
-                            }
-                            issued[side] = n + 1;
-                        }
-                    }
-                }
-                if (!ok) abort_flag = 1;
-                __syncwarp();
-                // after an abort the copies still in flight must land before the shared memory goes away
-                if (*abortp)
-                    for (int side = 0; side < 2; side++)
-                        for (uint32_t i = issued[side] > 2 ? issued[side] - 2 : 0; i < issued[side]; i++)
-                            mbar_wait(bar((side ? kVFull : kKFull) + (i & 1)), (i >> 1) & 1, &never);
-            }
-        } else {
-            // ---------------- values: 16 bytes of a position at once ----------------
-            constexpr int kRounds = P::kValueRounds;
-            const int first = tid - 13 * 32;
-            const uint8_t* mine = raw + P::kRawKeys + first * 16;            // a thread reads what it copied
-            const half2* my_par = reinterpret_cast<const half2*>(raw + P::kRawKeys + kRounds * kValueThreads * 16) + first;
-            Walk w(a, whole, lane);
-            uint32_t n = 0;
+        }
+        if (!ok) {
+            abort_flag = 1;
+            // what was issued completes before the memory is given up
+            commit(leader, bar(kLast + i));
+            __syncwarp();
+            mbar_wait(bar(kLast + i), 0, &never);
+        }
+    } else if (warp >= 8 && !UNPACK) {
+        if (warp == 8) {
+            // ---------------- copies of expanded keys and values ----------------
+            const bool leader = elect_one();
+            Walk w(a, whole, start);
+            uint32_t n = 0, issued[2] = {0, 0};
             bool ok = true;
             while (ok && w.advance()) {
-                const size_t row0 = cache_row(a.c, w.b, w.head, 0);
-                const auto load = [&](int j, int k) {
-                    const int e = first + k * kValueThreads, c = e / kTile, p = j * kTile + e % kTile;
-                    const bool valid = c < kCodes && p < w.visible;         // positions behind hold anything: they become 0
-                    const size_t at = row0 + (valid ? p : 0);
-                    copy_async<16>(smem_u32(mine) + k * kValueThreads * 16, a.c.vc + at * (DIM / 2) + (valid ? c * 16 : 0), valid);
-                    copy_async<4>(smem_u32(my_par) + k * kValueThreads * 4, a.c.vp + at * P::kBlocks + (valid ? c / 2 : 0), valid);
-                };
+                const int row0 = (w.b * w.kv_heads + w.head) * x.cap;
+                for (int j = w.j0; ok && j < w.j1; j++, n++) {
+                    const uint32_t st = n & 1, parity = ((n >> 1) & 1) ^ 1;
 #pragma unroll
-                for (int k = 0; k < kRounds; k++) load(w.j0, k);
-                for (int j = w.j0; j < w.j1; j++, n++) {
-                    const uint32_t st = n & 1;
-                    copies_landed();
-                    if (!(ok = mbar_wait(bar(kVEmpty + st), ((n >> 1) & 1) ^ 1, abortp))) break;
+                    for (int side = 0; side < 2; side++) {
+                        const uint32_t full = bar((side ? kVFull : kKFull) + st);
+                        if (!(ok = mbar_wait(bar((side ? kVEmpty : kKEmpty) + st), parity, abortp))) break;
+                        if (leader) {
+                            mbar_expect_tx(full, P::kOperand);
 #pragma unroll
-                    for (int k = 0; k < kRounds; k++) {
-                        const int e = first + k * kValueThreads, c = e / kTile;
-                        if (c < kCodes)
-                            unpack32(vs + st * P::kOperand, e % kTile, c * 4, *reinterpret_cast<const uint4*>(mine + k * kValueThreads * 16), my_par[k * kValueThreads]);
-                        if (j + 1 < w.j1) load(j + 1, k);
+                            for (int c = 0; c < P::kBlocks; c++)
+                                tma_load_2d(smem_u32((side ? vs : ks) + st * P::kOperand + c * kBlock), side ? &x.v : &x.k, c * 64, row0 + j * kTile, full);
+                        }
+                        issued[side] = n + 1;
                     }
-                    fence_async();
-                    mbar_arrive(bar(kVFull + st));
                 }
             }
-            copies_landed();
             if (!ok) abort_flag = 1;
+            __syncwarp();
+            // after an abort the copies still in flight must land before the shared memory goes away
+            if (*abortp)
+                for (int side = 0; side < 2; side++)
+                    for (uint32_t i = issued[side] > 2 ? issued[side] - 2 : 0; i < issued[side]; i++)
+                        mbar_wait(bar((side ? kVFull : kKFull) + (i & 1)), (i >> 1) & 1, &never);
         }
     } else if (warp >= 8) {
-        fewer_registers<kFew<UNPACK>>();
-        // ---------------- keys: a position a thread ----------------
-        if constexpr (UNPACK) {
-        const int row = tid - 256;
-        const uint8_t* mine = raw + row * 16;
-        const half2* my_par = reinterpret_cast<const half2*>(raw + kCodes * kTile * 16 + row * 4 * P::kBlocks);
-        Walk w(a, whole, lane);
+        // ---------------- unpacking: 16 bytes of a position at once ----------------
+        // A thread copies what it unpacks for the tile after this one (cp.async), and reads it back itself.
+        constexpr int kRounds = P::kRounds;
+        const int first = (warp < 12 ? warp - 8 : warp - 10) * 32 + lane;
+        Walk w(a, whole, start);
         uint32_t n = 0;
         bool ok = true;
         while (ok && w.advance()) {
             const size_t row0 = cache_row(a.c, w.b, w.head, 0);
-            const auto load = [&](int j, int c) {
-                const int p = j * kTile + row;
-                const bool valid = p < w.visible;
-                const size_t at = row0 + (valid ? p : 0);
-                copy_async<16>(smem_u32(mine) + c * kTile * 16, a.c.kc + at * (DIM / 2) + c * 16, valid);
-            };
-            const auto load_par = [&](int j) {
-                const int p = j * kTile + row;
-                const bool valid = p < w.visible;
-                copy_async<4 * P::kBlocks>(smem_u32(my_par), a.c.kp + (row0 + (valid ? p : 0)) * P::kBlocks, valid);
-            };
-            load_par(w.j0);
+            const auto load = [&](int side, int j) {
 #pragma unroll
-            for (int c = 0; c < kCodes; c++) load(w.j0, c);
-            for (int j = w.j0; j < w.j1; j++, n++) {
-                const uint32_t st = n & 1;
-                copies_landed();
-                if (!(ok = mbar_wait(bar(kKEmpty + st), ((n >> 1) & 1) ^ 1, abortp))) break;
-                half2 par[P::kBlocks];
-#pragma unroll
-                for (int c = 0; c < P::kBlocks; c++) par[c] = my_par[c];
-                if (j + 1 < w.j1) load_par(j + 1);
-#pragma unroll
-                for (int c = 0; c < kCodes; c++) {
-                    unpack32(ks + st * P::kOperand, row, c * 4, *reinterpret_cast<const uint4*>(mine + c * kTile * 16), par[c / 2]);
-                    if (j + 1 < w.j1) load(j + 1, c);
+                for (int k = 0; k < kRounds; k++) {
+                    const int e = first + k * kUnpackThreads, c = e / kTile, p = j * kTile + e % kTile;
+                    const bool valid = c < kCodes && p < w.visible;         // positions behind hold anything: they become 0
+                    const size_t at = row0 + (valid ? p : 0);
+                    const uint32_t to = smem_u32(raw + side * P::kRawSide);
+                    copy_async<16>(to + (first + k * kUnpackThreads) * 16, (side ? a.c.vc : a.c.kc) + at * (DIM / 2) + (valid ? c * 16 : 0), valid);
+                    copy_async<4>(to + kRounds * kUnpackThreads * 16 + (first + k * kUnpackThreads) * 4, (side ? a.c.vp : a.c.kp) + at * P::kBlocks + (valid ? c / 2 : 0), valid);
                 }
-                fence_async();
-                mbar_arrive(bar(kKFull + st));
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            load(0, w.j0);
+            load(1, w.j0);
+            for (int j = w.j0; ok && j < w.j1; j++, n++) {
+                const uint32_t st = n & 1, parity = ((n >> 1) & 1) ^ 1;
+#pragma unroll
+                for (int side = 0; side < 2; side++) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");    // the other side's copies are younger
+                    if (!(ok = mbar_wait(bar((side ? kVEmpty : kKEmpty) + st), parity, abortp))) break;
+                    const uint8_t* from = raw + side * P::kRawSide;
+#pragma unroll
+                    for (int k = 0; k < kRounds; k++) {
+                        const int e = first + k * kUnpackThreads, c = e / kTile;
+                        if (c < kCodes)
+                            unpack32((side ? vs : ks) + st * P::kOperand, e % kTile, c * 4, reinterpret_cast<const uint4*>(from)[e],
+                                     reinterpret_cast<const half2*>(from + kRounds * kUnpackThreads * 16)[e]);
+                    }
+                    fence_async();
+                    mbar_arrive(bar((side ? kVFull : kKFull) + st));
+                    if (j + 1 < w.j1) load(side, j + 1);
+                    else asm volatile("cp.async.commit_group;" ::: "memory");
+                }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
-        copies_landed();
         if (!ok) abort_flag = 1;
-        }
     } else {
-        more_registers<kMany<UNPACK>>();
         // ---------------- softmax: a row a thread ----------------
         const int i = warp >> 2, row = tid & (kTile - 1);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, row_s = tmem + i * kTile + lanes, row_o = tmem + kRowTiles * kTile + i * DIM + lanes;
-        Walk w(a, whole, lane);
-        if (!whole && tid == 0) entry_of(a.ws, blockIdx.x)->parts = 0;
+        Walk w(a, whole, start);
+        const bool wide = ((reinterpret_cast<uintptr_t>(out.p) | (uintptr_t)out.ld * sizeof(T)) & 31) == 0;     // outputs on whole sectors
         uint32_t rounds = 0;
         bool ok = true;
         while (ok && w.advance()) {
@@ -507,80 +481,64 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
             scale2 = fmaxf(scale2, 1e-37f);                                 // a masked score times it stays -infinity
             const f32x2 scale = pair_f32(scale2, scale2);
             float m = -INFINITY, l = 0.f;
-            for (int j = w.j0; j < w.j1; j++, rounds++) {
-                ok = __all_sync(0xffffffffu, mbar_wait(bar(kSFull + i), rounds & 1, abortp));
+            for (int j = 2 * w.j0; j < 2 * w.j1; j++) {
+                const int h = j & 1, u = i + 2 * h;
+                const uint32_t at_s = row_s + h * kHalf, parity = rounds & 1;
+                rounds += h;
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(kSFull + u), parity, abortp));
                 if (!ok) break;
                 fence_after();
-                uint32_t s[4][32];
-                tmem_ld32(row_s, s[0]);
-                tmem_ld32(row_s + 32, s[1]);
+                uint32_t s[2][32];
+                tmem_ld32(at_s, s[0]);
+                tmem_ld32(at_s + 32, s[1]);
                 wait_ld();
-                tmem_ld32(row_s + 64, s[2]);
-                tmem_ld32(row_s + 96, s[3]);
-                const bool masked = (j + 1) * kTile > least;                // some (row, position) of the tile is
-                const int seen = sees - j * kTile;
-                float top[2] = {-INFINITY, -INFINITY};
-                const auto mask = [&](int part) {
-                    if (masked)
+                if ((j + 1) * kHalf > least) {                              // some (row, position) is masked
+                    const int seen = sees - j * kHalf;
 #pragma unroll
-                        for (int k = 0; k < 64; k++)
-                            if (part * 64 + k >= seen) s[part * 2 + k / 32][k % 32] = 0xff800000u;
-                };
-                const auto largest = [&](int k) {                            // of four scores
-                    const uint32_t(&v)[32] = s[k / 32];
-                    top[0] = max3(top[0], __uint_as_float(v[k % 32]), __uint_as_float(v[k % 32 + 1]));
-                    top[1] = max3(top[1], __uint_as_float(v[k % 32 + 2]), __uint_as_float(v[k % 32 + 3]));
-                };
-                f32x2 sum[2], off;
+                    for (int k = 0; k < kHalf; k++)
+                        if (k >= seen) s[k / 32][k % 32] = 0xff800000u;
+                }
+                // With the maximum so far, which rarely has to move: the search for it runs beside the exponentials, and a second pass follows
+                // where it moved.
+                f32x2 sum[2];
                 uint32_t pw[32];
-                const auto weights = [&](int part, auto between) {           // of 64 positions
+#pragma unroll 1
+                for (int pass = 0; pass < 2; pass++) {
+                    const float ref = kLift - (m == -INFINITY ? 0.f : m);
+                    const f32x2 off = pair_f32(ref, ref);
+                    float top[2] = {-INFINITY, -INFINITY};
+                    sum[0] = sum[1] = 0ull;
 #pragma unroll
                     for (int k = 0; k < 32; k++) {
-                        const uint32_t(&v)[32] = s[part * 2 + k / 16];
-                        const float2 e = split_f32(fma_pairs(pair_f32(v[k % 16 * 2], v[k % 16 * 2 + 1]), scale, off));
-                        const float x = exp2_neg(e.x), y = exp2_neg(e.y);
-                        sum[k & 1] = add_pair(sum[k & 1], pair_f32(x, y));
-                        pw[k] = Pair2<half>::of(x, y);
-                        between(k);
+                        const uint32_t(&v)[32] = s[k / 16];
+                        const uint32_t v0 = v[k % 16 * 2], v1 = v[k % 16 * 2 + 1];
+                        const f32x2 e = fma_pairs(pair_f32(v0, v1), scale, off);
+                        f32x2 w;
+                        if (k % kEvery < kPolynomial) {
+                            w = exp2_pair(e);
+                        } else {
+                            const float2 x = split_f32(e);
+                            w = pair_f32(exp2_neg(x.x), exp2_neg(x.y));
+                        }
+                        sum[k & 1] = add_pair(sum[k & 1], w);
+                        const float2 y = split_f32(w);
+                        pw[k] = Pair2<half>::of(y.x, y.y);
+                        top[k & 1] = max3(top[k & 1], __uint_as_float(v0), __uint_as_float(v1));
                     }
-                };
-                const auto hand_over = [&](int part) {
-                    tmem_st32(row_s + part * 32, pw);
-                    wait_st();
-                    fence_before();
-                    mbar_arrive(bar(kPReady + 2 * i + part));
-                };
-                const auto reference = [&] {
-                    const float ref = kLift - (m == -INFINITY ? 0.f : m);
-                    off = pair_f32(ref, ref);
-                    sum[0] = sum[1] = 0ull;
-                };
-                mask(0);
-                // with the maximum so far, which rarely has to move: its own search runs beside the exponentials
-                const bool guess = !UNPACK && j > w.j0;
-                if (guess) {
-                    wait_ld();
-                    mask(1);
-                    reference();
-                    weights(0, [&](int k) { largest(4 * k); });
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 64; k += 4) largest(k);
-                    wait_ld();
-                    mask(1);
-#pragma unroll
-                    for (int k = 64; k < 128; k += 4) largest(k);
-                }
-                const float mx = fmaxf(top[0], top[1]) * scale2;
-                const bool grows = mx > m + kSlack;
-                const bool any = __any_sync(0xffffffffu, grows);
-                if (any) {
+                    const float mx = max3(top[0], top[0], top[1]) * scale2;
+                    if (pass || !__any_sync(0xffffffffu, !(mx <= m + kSlack))) break;
+                    const bool grows = mx > m + kSlack;
                     const float f = grows ? exp2_neg(m - mx) : 1.f;         // 0 where nothing was seen before
                     if (grows) {
                         m = mx;
                         l *= f;
                     }
-                    if (j > w.j0) {
+                    if (!(mx < INFINITY)) l = NAN;                          // a score that is no number
+                    if (j > 2 * w.j0) {
+                        // the output of the half before may be under way
+                        ok = __all_sync(0xffffffffu, mbar_wait(bar(kPvDone + i + 2 * (h ^ 1)), h ? parity : parity ^ 1, abortp));
+                        if (!ok) break;
+                        fence_after();
 #pragma unroll 1
                         for (int c = 0; c < DIM; c += 16) {
                             uint32_t o[16];
@@ -592,16 +550,14 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
                         }
                     }
                 }
-                if (any || !guess) {
-                    reference();
-                    weights(0, [](int) {});
-                }
-                hand_over(0);
-                weights(1, [](int) {});
-                hand_over(1);
+                if (!ok) break;
+                tmem_st32(at_s, pw);
                 l += sum_pair(add_pair(sum[0], sum[1]));
+                wait_st();
+                fence_before();
+                mbar_arrive(bar(kPReady + u));
             }
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(kPvDone + i), (rounds - 1) & 1, abortp));
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(kPvDone + i + 2), (rounds - 1) & 1, abortp));
             if (!ok) break;
             fence_after();
             T* y = out.p + (size_t)(w.span.row0 + token) * out.ld + (size_t)head * DIM;
@@ -610,26 +566,32 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
             float* rec = complete ? nullptr : record_of<DIM, kRows>(a.ws, gridDim.x, blockIdx.x, w.segment > 0);
             if (!complete && w.j0 == 0 && tid == 0)
                 *entry_of(a.ws, blockIdx.x) =
-                    Shared4{w.owner(w.x - 1, gridDim.x) - (int)blockIdx.x + 1, w.segment > 0, w.head, w.tile, w.span.row0, w.span.n, w.span.len, 0};
+                    Shared4{w.owner(w.x - 1) - (int)blockIdx.x + 1, w.segment > 0, w.head, w.tile, w.span.row0, w.span.n, w.span.len, 0};
             if (!complete && there) {
                 rec[at] = m;
                 rec[kRows + at] = l;
             }
+            const float f = sees > 0 ? 1.f / l : 0.f;
 #pragma unroll 1
             for (int c = 0; c < DIM; c += 32) {
                 uint32_t o[32];
                 tmem_ld32(row_o + c, o);
                 wait_ld();
-                if (there) {
-                    if (complete) {
+                if (there && complete) {
+                    uint32_t p[16];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            store_row<T>(y + c + e, make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])), l,
-                                         sees > 0);
+                    for (int e = 0; e < 16; e++)
+                        p[e] = sees > 0 ? Pair2<T>::of(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f) : 0u;
+                    if (wide) {
+                        store32(y + c, p);
+                        store32(y + c + 16, p + 8);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(rec + 2 * kRows + at * DIM + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        for (int e = 0; e < 4; e++) reinterpret_cast<uint4*>(y + c)[e] = make_uint4(p[4 * e], p[4 * e + 1], p[4 * e + 2], p[4 * e + 3]);
                     }
+                } else if (there) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) store32(rec + 2 * kRows + at * DIM + c + e, o + e);
                 }
             }
             fence_before();                                                 // the next products come after these reads

@@ -107,19 +107,19 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
     const int per = a.heads / a.c.kv_heads;
     pdl_wait();
 
-    if (blockIdx.x == 0 && warp == 0)
-        for (int b = lane; b < a.s.batch; b += 32) span_of(a.s, b, true);
-    Work<ROWS, kStepChunk> work(a.s, per, a.c.kv_heads, whole, lane);
-    const long long from = work.start(blockIdx.x, gridDim.x), to = work.start(blockIdx.x + 1, gridDim.x);
+    __shared__ typename Work<ROWS, kStepChunk>::Start start;
+    Work<ROWS, kStepChunk> work(a.s, per, a.c.kv_heads, whole);
+    if (warp == 0) work.find(blockIdx.x, gridDim.x, lane, &start);
     if (!whole && tid == 0) entry_of(a.ws, blockIdx.x)->parts = 0;
-    if (from >= to) return;
-    work.find(from, lane);
-    int segment = 0;
+    __syncthreads();
+    work.begin(start);
+    const int to = work.to;
 
-    for (long long x = from; x < to; segment++) {
+    int segment = 0;
+    for (int x = work.x; x < to; segment++) {
         // ---- the next head's rows and the part of its chunks ----
         const int chunks = work.chunks, units = work.kFixed + chunks;
-        const int j0 = whole ? 0 : work.chunk_at(work.offset), j1 = whole ? chunks : work.chunk_at(min((long long)units, work.offset + (to - x)));
+        const int j0 = whole ? 0 : work.chunk_at(work.offset), j1 = whole ? chunks : work.chunk_at(min(units, work.offset + (to - x)));
         x += whole ? 1 : units - work.offset;
         if (j0 == j1) {
             if (x < to) work.next();
@@ -440,7 +440,7 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
         const bool complete = j0 == 0 && j1 == chunks;
         float* rec = complete ? nullptr : record_of<DIM, ROWS>(a.ws, gridDim.x, blockIdx.x, segment > 0);
         if (!complete && j0 == 0 && tid == 0)
-            *entry_of(a.ws, blockIdx.x) = Shared4{work.owner(x - 1, gridDim.x) - (int)blockIdx.x + 1, segment > 0, work.head, work.tile, sp.row0, sp.n, sp.len, 0};
+            *entry_of(a.ws, blockIdx.x) = Shared4{work.owner(x - 1) - (int)blockIdx.x + 1, segment > 0, work.head, work.tile, sp.row0, sp.n, sp.len, 0};
         for (int e = tid; e < tile_rows * (DIM / 4); e += kThreads) {
             const int r = e / (DIM / 4), c = e % (DIM / 4) * 4;
             float top = -INFINITY;

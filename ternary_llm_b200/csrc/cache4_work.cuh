@@ -53,36 +53,55 @@ int launch_cache4_join(const Cache4Call& a, Rows<T> out, int rows, int ctas, cud
 #ifdef __CUDACC__
 // Row r of sequence b and key/value head `head` is query head r % per of the head's, of new token r / per; a tile is R of
 // them.  Units are whole tiles, or chunks of positions behind kFixed units a tile (its rows' loading, joining and
-// storing, in chunks), so that CTAs with many short tiles and CTAs with a part of a long one take equally long.  Members are
-// found by whole warps, every lane with the same result.
+// storing, in chunks), so that CTAs with many short tiles and CTAs with a part of a long one take equally long; a CTA takes
+// `share` units in a row.  One warp finds a CTA's first unit (its lanes share sequences or tiles), all threads walk on from there.
+// Units are counted in 32 bits (work_fits).
 template <int R, int CHUNK>
 struct Work {
     static constexpr int kFixed = CHUNK == kStepChunk ? 8 : 2;
     static constexpr int kLeast = CHUNK == kStepChunk ? 24 : 4;            // units that a CTA takes at least where work is cut
+    struct Start {
+        int x, to, share, b, head, tile, offset;
+    };
     Seqs s;
     int per, kv_heads;
     bool whole;
-    long long total;
-    // the unit that find() or next() came to
-    int b, head, tile, offset, rows, chunks, visible;
+    // the CTA's units, and the tile that begin() or next() came to
+    int x, to, share, b, head, tile, offset, rows, chunks, visible;
     Span span;
 
+    __device__ __forceinline__ Work(const Seqs& s_, int per_, int kv_heads_, bool whole_) : s(s_), per(per_), kv_heads(kv_heads_), whole(whole_) {}
     __device__ __forceinline__ int seen(const Span& sp, int tl) const      // positions that some row of a tile sees
     {
         const int last = min((tl + 1) * R, sp.n * per) - 1;
         return max(sp.position(last / per) + 1, 0);
     }
     __device__ __forceinline__ int chunks_of(const Span& sp, int tl) const { return max((seen(sp, tl) + CHUNK - 1) / CHUNK, 1); }
-    __device__ __forceinline__ int units_of(const Span& sp, int tl) const { return kFixed + chunks_of(sp, tl); }
-    // the first chunk at or behind unit u of a tile, and the unit where it begins
-    static __device__ __forceinline__ int chunk_at(long long u) { return u > kFixed ? (int)u - kFixed : 0; }
-    __device__ __forceinline__ int tiles_of(const Span& sp) const { return (int)(((long long)sp.n * per + R - 1) / R); }
-    // units of a head of each lane's sequence; the lanes share the tiles of one where there are many
-    __device__ __forceinline__ long long units(const Span& sp, int lane) const
+    __device__ __forceinline__ int units_of(const Span& sp, int tl) const { return whole ? 1 : kFixed + chunks_of(sp, tl); }
+    // the first chunk at or behind unit u of a tile
+    static __device__ __forceinline__ int chunk_at(int u) { return max(u - kFixed, 0); }
+    __device__ __forceinline__ int tiles_of(const Span& sp) const { return (sp.n * per + R - 1) / R; }
+    __device__ __forceinline__ Span lane_span(int i) const
+    {
+        Span none;
+        none.row0 = none.n = none.len = 0;
+        return i < s.batch ? span_of(s, i, false) : none;
+    }
+    static __device__ __forceinline__ int scan(int v, int lane)
+    {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int w = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += w;
+        }
+        return v;
+    }
+    // units of a head of each lane's sequence
+    __device__ __forceinline__ int units(const Span& sp, int lane) const
     {
         const int tiles = tiles_of(sp);
         if (whole) return tiles;
-        long long sum = 0;
+        int sum = 0;
         if (__all_sync(0xffffffffu, tiles <= 2)) {
             for (int i = 0; i < tiles; i++) sum += units_of(sp, i);
             return sum;
@@ -92,97 +111,77 @@ struct Work {
             Span one;
             one.n = __shfl_sync(0xffffffffu, sp.n, from);
             one.len = __shfl_sync(0xffffffffu, sp.len, from);
-            long long part = 0;
+            int part = 0;
             for (int i = lane; i < n; i += 32) part += units_of(one, i);
-            part = warp_total(part);
+            part = __reduce_add_sync(0xffffffffu, part);
             if (lane == from) sum = part;
         }
         return sum;
     }
-    static __device__ __forceinline__ long long warp_total(long long v)
+    // by one warp: where part c of `parts` begins, and reports what is wrong with the sequences
+    __device__ __forceinline__ void find(int c, int parts, int lane, Start* out) const
     {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        return v;
-    }
-    static __device__ __forceinline__ long long warp_scan(long long v, int lane)
-    {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long w = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += w;
+        int total = 0;
+        for (int b0 = 0; b0 < s.batch; b0 += 32) {
+            if (c == 0 && b0 + lane < s.batch) span_of(s, b0 + lane, true);
+            total += __reduce_add_sync(0xffffffffu, units(lane_span(b0 + lane), lane) * kv_heads);
         }
-        return v;
+        Start r;
+        r.share = max((total + parts - 1) / parts, whole ? 1 : kLeast);
+        r.x = min((long long)c * r.share, (long long)total);
+        r.to = min(r.x + r.share, total);
+        r.b = r.head = r.tile = r.offset = 0;
+        if (r.x < r.to) {
+            int at = r.x, u = 0;                      // u: units of a head of the sequence
+            for (int b0 = 0; b0 < s.batch; b0 += 32) {
+                const int mine = units(lane_span(b0 + lane), lane), up_to = scan(mine * kv_heads, lane);
+                const uint32_t m = __ballot_sync(0xffffffffu, up_to > at);
+                const int i = m ? __ffs(m) - 1 : 31, end = __shfl_sync(0xffffffffu, up_to, i);
+                u = __shfl_sync(0xffffffffu, mine, i);
+                at -= m ? end - u * kv_heads : end;
+                r.b = b0 + i;
+                if (m) break;
+            }
+            const Span sp = span_of(s, r.b, false);
+            r.head = at / u;
+            at -= r.head * u;
+            const int tiles = tiles_of(sp);
+            for (;; r.tile += 32) {
+                const int mine = r.tile + lane < tiles ? units_of(sp, r.tile + lane) : 0, up_to = scan(mine, lane);
+                const uint32_t m = __ballot_sync(0xffffffffu, up_to > at);
+                const int i = m ? __ffs(m) - 1 : 31, end = __shfl_sync(0xffffffffu, up_to, i);
+                at -= m ? end - __shfl_sync(0xffffffffu, mine, i) : end;
+                if (m) {
+                    r.tile += i;
+                    break;
+                }
+            }
+            r.offset = at;
+        }
+        if (lane == 0) *out = r;
     }
-    __device__ __forceinline__ Span lane_span(int i) const
-    {
-        Span none;
-        none.row0 = none.n = none.len = 0;
-        return i < s.batch ? span_of(s, i, false) : none;
-    }
-    __device__ __forceinline__ Work(const Seqs& s_, int per_, int kv_heads_, bool whole_, int lane) : s(s_), per(per_), kv_heads(kv_heads_), whole(whole_), total(0)
-    {
-        for (int b0 = 0; b0 < s.batch; b0 += 32) total += units(lane_span(b0 + lane), lane) * kv_heads;
-        total = warp_total(total);
-    }
-    // first unit of part c of `parts`
-    __device__ __forceinline__ int used(int parts) const
-    {
-        if (whole) return parts;
-        const long long most = total / kLeast;
-        return most < 1 ? 1 : most < parts ? (int)most : parts;
-    }
-    __device__ __forceinline__ long long start(int c, int parts) const
-    {
-        const int n = used(parts);
-        return c >= n ? total : total * c / n;
-    }
-    __device__ __forceinline__ int owner(long long x, int parts) const { return (int)(((x + 1) * used(parts) - 1) / total); }
-
     __device__ __forceinline__ void set_tile(int tl)
     {
         tile = tl;
         visible = seen(span, tl);
         chunks = max((visible + CHUNK - 1) / CHUNK, 1);
     }
-    // unit x < total
-    __device__ __forceinline__ void find(long long x, int lane)
+    __device__ __forceinline__ void begin(const Start& f)
     {
-        long long u = 0;                              // of a head of the sequence
-        for (int b0 = 0; b0 < s.batch; b0 += 32) {
-            const long long mine = units(lane_span(b0 + lane), lane), up_to = warp_scan(mine * kv_heads, lane);
-            const uint32_t m = __ballot_sync(0xffffffffu, up_to > x);
-            const int at = m ? __ffs(m) - 1 : 31;
-            u = __shfl_sync(0xffffffffu, mine, at);
-            const long long end = __shfl_sync(0xffffffffu, up_to, at);
-            x -= m ? end - u * kv_heads : end;
-            b = b0 + at;
-            if (m) break;
+        x = f.x;
+        to = f.to;
+        share = f.share;
+        b = f.b;
+        head = f.head;
+        offset = f.offset;
+        if (x < to) {
+            span = span_of(s, b, false);
+            rows = span.n * per;
+            set_tile(f.tile);
         }
-        span = span_of(s, b, false);
-        rows = span.n * per;
-        head = (int)(x / u);
-        x -= head * u;
-        int tl = 0;
-        offset = 0;
-        if (whole) tl = (int)x;
-        else {
-            const int tiles = tiles_of(span);
-            for (;; tl += 32) {
-                const long long mine = tl + lane < tiles ? units_of(span, tl + lane) : 0, up_to = warp_scan(mine, lane);
-                const uint32_t m = __ballot_sync(0xffffffffu, up_to > x);
-                const int at = m ? __ffs(m) - 1 : 31;
-                const long long end = __shfl_sync(0xffffffffu, up_to, at);
-                x -= m ? end - __shfl_sync(0xffffffffu, mine, at) : end;
-                if (m) {
-                    tl += at;
-                    break;
-                }
-            }
-            offset = (int)x;
-        }
-        set_tile(tl);
     }
+    // the CTA that has unit u
+    __device__ __forceinline__ int owner(int u) const { return u / share; }
     // the tile behind this one
     __device__ __forceinline__ void next()
     {
@@ -200,6 +199,12 @@ struct Work {
         set_tile(0);
     }
 };
+// Whether the units of a call fit 31 bits, whatever first and lens hold (even all rows in every sequence).
+inline bool work_fits(const Cache4& c, int tokens, int heads, int rows, int chunk)
+{
+    const double tiles = (double)tokens * (heads / c.kv_heads) / rows + 1, units = (double)c.rows / chunk + 10;
+    return tiles * units * c.batch * c.kv_heads < 2e9;
+}
 
 template <typename T> struct Pair2;
 template <> struct Pair2<half> {
@@ -223,6 +228,12 @@ __device__ __forceinline__ void store_row(T* p, float4 y, float sum, bool sees)
     const float f = sees ? 1.f / sum : 0.f;
     if (!sees) y = make_float4(0.f, 0.f, 0.f, 0.f);
     *reinterpret_cast<uint2*>(p) = make_uint2(Pair2<T>::of(y.x * f, y.y * f), Pair2<T>::of(y.z * f, y.w * f));
+}
+// A whole sector at once, on a 32-byte boundary.
+__device__ __forceinline__ void store32(void* p, const uint32_t* v)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 #endif
 
