@@ -197,7 +197,10 @@ def host():
         h = lib()
         address = [ctypes.cast(getattr(h, name), _vp).value for name in
                    ("tllm_b200_gemv_packed", "tllm_b200_gemv_int8_packed", "tllm_b200_gemm_packed")]
+        cache4 = [ctypes.cast(getattr(h, "tllm_b200_" + name), _vp).value for name in
+                  ("rotary", "cache4_append", "cache4_read", "cache4_attention", "cache4_workspace")]
         _hostcall.bind(*address, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.float16, torch.int8, torch.uint8)
+        _hostcall.bind_cache4(*cache4, torch.bfloat16, torch.float32, torch.int32)
         _host = _hostcall
     return _host
 

@@ -26,6 +26,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libtllm_b200.so")
 HOST_SRC, HOST_LIB = os.path.join(PKG, "csrc", "hostcall.c"), os.path.join(PKG, "_hostcall.so")
+HOST_INCLUDE = os.path.join(ROOT, "include", "tllm_b200_cache4.h")
 OBJ_DIR = os.path.join(ROOT, "build")
 
 NVCC_FLAGS = [
@@ -50,7 +51,7 @@ def _older(target: str, deps) -> bool:
 
 
 def _stale() -> bool:
-    return _older(LIB, sources() + headers()) or _older(HOST_LIB, [HOST_SRC])
+    return _older(LIB, sources() + headers()) or _older(HOST_LIB, [HOST_SRC, HOST_INCLUDE])
 
 
 def build(force: bool = False, verbose: bool = False, timeline: bool = False) -> str:
@@ -79,9 +80,10 @@ def build(force: bool = False, verbose: bool = False, timeline: bool = False) ->
         part = out + ".part"
         subprocess.check_call(["nvcc"] + NVCC_FLAGS[:2] + ["-shared", "-o", part] + [obj for _, obj in jobs])
         os.replace(part, out)
-        if force or _older(HOST_LIB, [HOST_SRC]):
+        if force or _older(HOST_LIB, [HOST_SRC, HOST_INCLUDE]):
             part = HOST_LIB + ".part"
-            subprocess.check_call(["gcc", "-O2", "-Wall", "-shared", "-fPIC", "-I" + sysconfig.get_paths()["include"], "-o", part, HOST_SRC])
+            subprocess.check_call(["gcc", "-O2", "-Wall", "-shared", "-fPIC", "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(ROOT, "include"),
+                                   "-o", part, HOST_SRC])
             os.replace(part, HOST_LIB)
     return out
 

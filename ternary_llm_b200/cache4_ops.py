@@ -49,9 +49,13 @@ def rotary_frequencies(rot_dim: int, base: float, scaling: dict | None = None):
 def rotary_turns(frequencies):
     """The frequencies in turns a position, as 64-bit fractions."""
     n = len(frequencies)
+    return list(_turns(frequencies, n))[:n]
+
+
+def _turns(frequencies, n: int):
     out = (ctypes.c_uint64 * max(1, n))()
     _lib.check(_lib.lib().tllm_b200_rotary_turns((ctypes.c_double * max(1, n))(*frequencies), n, out))
-    return list(out)[:n]
+    return out
 
 
 class RotaryTable:
@@ -68,8 +72,10 @@ class RotaryTable:
                 raise ValueError(f"{len(frequencies)} frequencies for {rot_dim} entries")
         self.rot_dim, self.half, self.frequencies = rot_dim, half, frequencies
         self.amplitude = own if amplitude is None else float(amplitude)
-        turns = [t - 2 ** 64 if t >= 2 ** 63 else t for t in rotary_turns(frequencies)]
-        self.turns = torch.tensor(turns, dtype=torch.int64, device="cuda" if device is None else device)
+        turns = _turns(frequencies, rot_dim // 2)
+        self.turns = torch.frombuffer(turns, dtype=torch.int64, count=rot_dim // 2).to("cuda" if device is None else device, copy=True)
+        self._device = self.turns.get_device()
+        self._bytes = bytes(_lib.RotaryTableDesc(self.turns.data_ptr(), rot_dim, int(half), self.amplitude))
 
     def _desc(self):
         return _lib.RotaryTableDesc(_chk(self.turns, torch.int64, "turns", self.rot_dim // 2), self.rot_dim, int(self.half), self.amplitude)
@@ -90,6 +96,12 @@ class Cache4:
             if tuple(t.shape) != tuple(shape):
                 raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
+        # for the native calls; any other device or layout goes through _desc, which says what is wrong
+        all4 = (k_codes, k_params, v_codes, v_params)
+        fit = k_codes.is_cuda and all(t.is_contiguous() and t.device == k_codes.device for t in all4) and \
+            k_codes.dtype == v_codes.dtype == torch.uint8 and k_params.dtype == v_params.dtype == torch.float16
+        self._device = k_codes.get_device() if fit else -1
+        self._bytes = bytes(_lib.Cache4Desc(*(t.data_ptr() for t in all4), self.batch, self.kv_heads, self.rows, self.dim)) if fit else b""
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, rows: int, dim: int, device=None):
@@ -136,6 +148,9 @@ def _ref(d):
 def rotary(q, k, positions, table: RotaryTable, q_out=None, k_out=None, inverse: bool = False) -> None:
     """Turns q [tokens, heads, dim] and k [tokens, kv_heads, dim] (or None) by positions int32 [tokens], in place where no
     output is given; inverse turns back (the gradient).  FP16, BF16 or FP32."""
+    st = _lib.host().rotary(table._bytes, table._device, q, k, positions, q_out, k_out, inverse)
+    if st is not None:
+        return _lib.check(st)
     kind = _type(q, "q", tuple(TYPES))
     tokens, heads, dim = q.shape
     if k is None and k_out is not None:
@@ -150,6 +165,10 @@ def rotary(q, k, positions, table: RotaryTable, q_out=None, k_out=None, inverse:
 
 def append(cache: Cache4, q, k, v, first, lens, table: RotaryTable | None = None, q_out=None) -> None:
     """Turns q (or None) into q_out (default: in place) and k, and writes k and v to the cache.  FP16 or BF16."""
+    st = _lib.host().cache4_append(cache._bytes, cache._device, None if table is None else table._bytes, 0 if table is None else table._device, q, k, v,
+                                   first, lens, q_out)
+    if st is not None:
+        return _lib.check(st)
     kind = _type(k, "k", (torch.float16, torch.bfloat16))
     tokens, d = k.shape[0], cache._desc()
     if q is None and q_out is not None:
@@ -166,6 +185,9 @@ def append(cache: Cache4, q, k, v, first, lens, table: RotaryTable | None = None
 def read(cache: Cache4, k, v, first, lens) -> None:
     """Writes the keys and values at the rows' positions, as the cache holds them, to k and v [tokens, kv_heads, dim] (one of
     them may be None).  FP16, BF16 or FP32."""
+    st = _lib.host().cache4_read(cache._bytes, cache._device, k, v, first, lens)
+    if st is not None:
+        return _lib.check(st)
     some = v if k is None else k
     if some is None:
         raise ValueError("neither k nor v")
@@ -180,6 +202,11 @@ def attention(cache: Cache4, q, out, first, lens, scale: float | None = None, ma
     """out = softmax(scale q k') v over the positions up to each row's own (scale: dim ** -0.5).  max_new: about the most rows
     of a sequence, 0 where the caller does not know; results do not depend on it but for the order of sums.  max_len: no
     sequence holds more positions (0: the cache's rows); workspaces are as large as that needs.  FP16 or BF16."""
+    if scale is None:
+        scale = cache.dim ** -0.5
+    st = _lib.host().cache4_attention(cache._bytes, cache._device, q, out, first, lens, scale, max_new, max_len)
+    if st is not None:
+        return _lib.check(st)
     kind, d = _type(q, "q", (torch.float16, torch.bfloat16)), cache._desc()
     tokens, heads = q.shape[:2]
     x, y = _rows(q, q.dtype, "q", tokens, heads, cache.dim), _rows(out, q.dtype, "out", tokens, heads, cache.dim)
@@ -188,5 +215,5 @@ def attention(cache: Cache4, q, out, first, lens, scale: float | None = None, ma
     _lib.check(h.tllm_b200_cache4_workspace(ctypes.byref(d), tokens, heads, max_new, max_len, ctypes.byref(need)))
     ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
     _lib.check(h.tllm_b200_cache4_attention(
-        ctypes.byref(d), kind, f, n, tokens, ctypes.byref(x), ctypes.byref(y), heads, cache.dim ** -0.5 if scale is None else scale, max_new,
-        max_len, None if ws is None else ws.data_ptr(), need.value, _stream()))
+        ctypes.byref(d), kind, f, n, tokens, ctypes.byref(x), ctypes.byref(y), heads, scale, max_new, max_len,
+        None if ws is None else ws.data_ptr(), need.value, _stream()))

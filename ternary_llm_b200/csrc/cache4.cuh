@@ -56,18 +56,6 @@ __device__ __forceinline__ Span span_of(const Seqs& s, int b, bool report)
     if (report && (lo < 0 || hi > s.tokens || hi < lo || len < 0 || len > s.rows)) atomicExch(s.err, TLLM_ERR_SHAPE);
     return r;
 }
-// The sequence that a row belongs to, found by one warp: the first whose end lies behind it; s.batch for none.
-__device__ __forceinline__ int seq_of_row(const Seqs& s, int row, int lane)
-{
-    if (row < s.first[0]) return s.batch;
-    for (int b0 = 0; b0 < s.batch; b0 += 32) {
-        const bool behind = b0 + lane < s.batch && row < s.first[b0 + lane + 1];
-        const uint32_t m = __ballot_sync(0xffffffffu, behind);
-        if (m) return b0 + __ffs(m) - 1;
-    }
-    return s.batch;
-}
-
 // Angle of a pair at a position: the position times the turns a position, as 64-bit fractions of a turn,
 // is exact modulo whole turns; its upper 32 bits are the angle to 2^-32 of a turn.
 __device__ __forceinline__ void turn(const Rotary& r, unsigned long long turns, int position, float& c, float& s)
@@ -78,6 +66,10 @@ __device__ __forceinline__ void turn(const Rotary& r, unsigned long long turns, 
     s *= r.inverse ? -r.amplitude : r.amplitude;
 }
 
+// The turned pair; written out, so that every kernel rounds alike.
+__device__ __forceinline__ float turned_first(float x1, float x2, float2 c) { return fmaf(x1, c.x, -(x2 * c.y)); }
+__device__ __forceinline__ float turned_second(float x1, float x2, float2 c) { return fmaf(x2, c.x, x1 * c.y); }
+
 template <typename T> __device__ __forceinline__ float as_float(T x);
 template <> __device__ __forceinline__ float as_float<half>(half x) { return __half2float(x); }
 template <> __device__ __forceinline__ float as_float<bf16>(bf16 x) { return __bfloat162float(x); }
@@ -86,6 +78,80 @@ template <typename T> __device__ __forceinline__ T as_type(float x);
 template <> __device__ __forceinline__ half as_type<half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ bf16 as_type<bf16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ float as_type<float>(float x) { return x; }
+
+// 16 bytes of activations as FP32 numbers.
+template <typename T>
+struct Vec {
+    static constexpr int n = 16 / sizeof(T);
+    float v[n];
+    __device__ __forceinline__ void load(const T* p)
+    {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+        for (int i = 0; i < n; i++) v[i] = as_float(e[i]);
+    }
+    __device__ __forceinline__ void store(T* p) const
+    {
+        uint4 x;
+        T* e = reinterpret_cast<T*>(&x);
+#pragma unroll
+        for (int i = 0; i < n; i++) e[i] = as_type<T>(v[i]);
+        *reinterpret_cast<uint4*>(p) = x;
+    }
+};
+
+// The rotation of a head in units of 16 bytes.  Half layout with pairs in whole units: unit u < pairs / n is two, u and u + pairs / n, which
+// turn together; other units are one each.  cs: cos and sin of the pairs at a position.
+template <typename T>
+struct Turn {
+    static constexpr int n = Vec<T>::n;
+    int pairs, together, per_head;     // units that hold two, units of a head
+    bool half_layout;
+    __host__ __device__ Turn(const Rotary& r, int dim) : pairs(r.rot / 2), half_layout(r.half_layout)
+    {
+        together = half_layout ? pairs / n : 0;
+        per_head = dim / n - together;
+    }
+    static bool whole(const Rotary& r) { return !r.half_layout || r.rot / 2 % n == 0; }
+    // requests unit u of a head
+    __device__ __forceinline__ void load(const T* x, int u, uint4 (&w)[2]) const
+    {
+        const int at = u < together ? u : u + together;
+        w[0] = reinterpret_cast<const uint4*>(x)[at];
+        if (u < together) w[1] = reinterpret_cast<const uint4*>(x)[u + together];
+    }
+    __device__ __forceinline__ void turn_and_store(T* y, int u, const uint4 (&w)[2], const float2* cs) const
+    {
+        Vec<T> a, b;
+        a.load(reinterpret_cast<const T*>(&w[0]));
+        if (u < together) {
+            b.load(reinterpret_cast<const T*>(&w[1]));
+#pragma unroll
+            for (int i = 0; i < n; i++) {
+                const float2 c = cs[u * n + i];
+                const float x1 = a.v[i], x2 = b.v[i];
+                a.v[i] = turned_first(x1, x2, c);
+                b.v[i] = turned_second(x1, x2, c);
+            }
+            a.store(y + u * n);
+            b.store(y + (u + together) * n);
+            return;
+        }
+        const int at = u + together;
+        if (!half_layout) {
+#pragma unroll
+            for (int i = 0; i < n; i += 2)
+                if (at * n + i < 2 * pairs) {
+                    const float2 c = cs[(at * n + i) / 2];
+                    const float x1 = a.v[i], x2 = a.v[i + 1];
+                    a.v[i] = turned_first(x1, x2, c);
+                    a.v[i + 1] = turned_second(x1, x2, c);
+                }
+        }
+        a.store(y + at * n);
+    }
+};
 
 // First element of a row of the cache, in groups of 64 values.
 __device__ __forceinline__ size_t cache_row(const Cache4& c, int b, int g, int row) { return ((size_t)b * c.kv_heads + g) * c.rows + row; }

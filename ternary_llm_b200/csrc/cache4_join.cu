@@ -38,6 +38,13 @@ cache4_join_kernel(const Cache4Call a, const Rows<T> out, const int ctas)
         store_row<T>(out.p + (size_t)(tile.row0 + i) * out.ld + (size_t)head * DIM + col, y, sums[r], tile.len - tile.n + i >= 0);
     };
 
+    constexpr int kAhead = 8;                                               // outputs requested before the weights are known
+    const int e0 = tid % (kParts > 1 ? kElems : kThreads), part = kParts > 1 ? tid / kElems : 0;
+    const auto output = [&](int e, int i) { return *reinterpret_cast<const float4*>(at(i) + 2 * ROWS + (r0 + e / (DIM / 4)) * DIM + e % (DIM / 4) * 4); };
+    float4 ahead[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; k++)
+        if (e0 < rows * (DIM / 4) && part + k * kParts < n) ahead[k] = output(e0, part + k * kParts);
     for (int r = warp; r < rows; r += kThreads / 32) {
         float m = -INFINITY, l = 0.f;
         for (int i = lane; i < n; i += 32) m = fmaxf(m, at(i)[r0 + r]);
@@ -52,15 +59,21 @@ cache4_join_kernel(const Cache4Call a, const Rows<T> out, const int ctas)
         if (lane == 0) sums[r] = l;
     }
     __syncthreads();
-    for (int e = tid % (kParts > 1 ? kElems : kThreads); e < rows * (DIM / 4); e += kParts > 1 ? kElems : kThreads) {
-        const int r = e / (DIM / 4), col = e % (DIM / 4) * 4, part = kParts > 1 ? tid / kElems : 0;
+    for (int e = e0; e < rows * (DIM / 4); e += kParts > 1 ? kElems : kThreads) {
+        const int r = e / (DIM / 4), col = e % (DIM / 4) * 4;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int i = part; i < n; i += kParts) {
-            const float4 v = *reinterpret_cast<const float4*>(at(i) + 2 * ROWS + (r0 + r) * DIM + col);
+        const auto add = [&](float4 v, int i) {
             const float w = weight[r][i];
             y = make_float4(fmaf(v.x, w, y.x), fmaf(v.y, w, y.y), fmaf(v.z, w, y.z), fmaf(v.w, w, y.w));
+        };
+        int i = part;
+        if (e == e0) {
+#pragma unroll
+            for (int k = 0; k < kAhead; k++, i += kParts)
+                if (i < n) add(ahead[k], i);
         }
+#pragma unroll 8
+        for (; i < n; i += kParts) add(output(e, i), i);
         if (kParts > 1) parts[tid] = y;
         else store(r, col, y);
     }

@@ -1,15 +1,15 @@
 // Attention over the 4-bit key/value cache for many rows a sequence, on the 5th-generation tensor cores.
 //
 // A CTA takes 256 rows of a key/value head (new tokens times the query heads that share it) as two tiles of 128 and
-// walks over tiles of 128 positions.  Roles: six warps turn codes into FP16 numbers in shared memory, rounded once
-// (l + s c, 11 bits); one for each tile of rows issues tcgen05.mma; four for each tile of rows have a row a thread.
+// walks over tiles of 128 positions.  Roles: three warps turn codes of keys into FP16 numbers in shared memory, rounded
+// once (l + s c, 11 bits), three those of values; one for each tile of rows issues tcgen05.mma; four for each tile of rows have a row a thread.
 //   S = Q K^T    both operands in shared memory, 128 FP32 columns of tensor memory for each tile of rows
 //   softmax      a thread reads its row; the weights go back over S as FP16, with a factor of 2^6 that leaves small
 //                ones their bits (the sum of the weights takes it out)
 //   O += P V     weights from tensor memory, values feature-major
 // so a tile of the cache is unpacked once for 256 rows, and one tile's products run beside the other's softmax.
-// BF16 queries become FP16 numbers times a power of two of their row.  The running maximum moves when it grows by more
-// than 2^8; sums are FP32.  A position that a row does not see is masked before the maximum, and values are finite
+// BF16 queries become FP16 numbers times a power of two of their row.  The running maximum moves when the weights of 64
+// positions add up to more than 2^8 of its own; sums are FP32.  A position that a row does not see is masked before the maximum, and values are finite
 // (append marks a NaN in the key), so nothing behind a row's own position reaches it.
 //
 // Work: tiles of rows, longest first; or, where there are too few, all tiles of positions as one sequence of which
@@ -32,10 +32,10 @@ using namespace gemm;
 
 constexpr int kTile = kPromptChunk, kRows = kPromptRows, kRowTiles = kRows / kTile;
 constexpr int kThreads = 512;                        // warps: softmax of a tile of rows 0-3, of the other 4-7, its products 12, 13, keys and values the rest
-constexpr int kUnpackThreads = 192;
+constexpr int kUnpackThreads = 96;                   // of keys, and of values
 constexpr int kBlock = kTile * 128;                  // bytes of 64 columns of a tile: 128-byte rows
 constexpr int kStages = 2, kHalf = kTile / 2;
-constexpr float kSlack = 8.f, kLift = 6.f, kLog2e = 1.4426950408889634f;
+constexpr float kLift = 6.f, kMost = 16384.f, kLog2e = 1.4426950408889634f;          // kMost: 2^8 times what kLift lifts
 
 template <int DIM>
 struct Prompt {
@@ -112,18 +112,11 @@ __device__ __forceinline__ f32x2 fma_pairs(f32x2 a, f32x2 b, f32x2 c)
     fma_pair(c, a, b);
     return c;
 }
-__device__ __forceinline__ f32x2 neg_pair(f32x2 v) { return v ^ 0x8000000080000000ull; }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// Keys and values as FP16 rows: [batch * kv_heads][cap][dim].
-struct Expanded {
-    CUtensorMap k, v;
-    int cap;
-};
 
 // A tile's rows of a key/value head and the tiles of positions [j0, j1) of its `chunks`, one after the other for this CTA;
 // every role walks over the same.
@@ -178,25 +171,8 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// Of every kEvery pairs of weights kPolynomial come from multiplications and additions, the others from the unit of special
-// functions, which takes a warp's instruction every eight clocks and would be the limit.
-constexpr int kEvery = 4, kPolynomial = 0;
-// 2^x of two numbers: x = n + f with n = rint(x) in the low bits of x + 1.5 * 2^23, a polynomial in f (|f| <= 1/2, of degree 4 with the
-// smallest largest relative error, 2.6e-6), and n added to the exponent.  Below -126: 2^-126.  A NaN gives any number.
-__device__ __forceinline__ f32x2 exp2_pair(f32x2 v)
-{
-    float2 x = split_f32(v);
-    v = pair_f32(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-    const f32x2 magic = pair_f32(12582912.f, 12582912.f), t = add_pair(v, magic), f = add_pair(v, neg_pair(add_pair(t, neg_pair(magic))));
-    f32x2 p = fma_pairs(f, pair_f32(0.009570102207362652f, 0.009570102207362652f), pair_f32(0.05591785907745361f, 0.05591785907745361f));
-    p = fma_pairs(p, f, pair_f32(0.240247443318367f, 0.240247443318367f));
-    p = fma_pairs(p, f, pair_f32(0.6931217908859253f, 0.6931217908859253f));
-    p = fma_pairs(p, f, pair_f32(0.9999992847442627f, 0.9999992847442627f));
-    const float2 n = split_f32(t), y = split_f32(p);
-    return pair_f32(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23), __float_as_uint(y.y) + (__float_as_uint(n.y) << 23));
-}
-// 32 codes as l + s c, rounded to FP16.
-__device__ __forceinline__ void expand32(const uint4& code, half2 par, uint4 (&y)[4])
+// 32 codes of a row as l + s c, rounded to FP16, to four 16-byte pieces of a tile at `dst`, exchanged as `turn` says.
+__device__ __forceinline__ void unpack32(uint32_t dst, uint32_t turn, const uint4& code, half2 par)
 {
     const half2 one = __halves2half2(__ushort_as_half(0x6400), __ushort_as_half(0x6400));
     const half2 sixteenth = __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00)), off = __halves2half2(__ushort_as_half(0xd400), __ushort_as_half(0xd400));
@@ -204,31 +180,22 @@ __device__ __forceinline__ void expand32(const uint4& code, half2 par, uint4 (&y
     const uint32_t word[4] = {code.x, code.y, code.z, code.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        half2 h[4];
+        uint32_t h[4];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const uint32_t v = k ? word[i] >> 8 : word[i], lo = (v & 0x000f000fu) | 0x64006400u, hi = (v & 0x00f000f0u) | 0x64006400u;
-            h[2 * k] = __hfma2(__hsub2(*reinterpret_cast<const half2*>(&lo), one), s, l);
-            h[2 * k + 1] = __hfma2(__hfma2(*reinterpret_cast<const half2*>(&hi), sixteenth, off), s, l);
+            const half2 x = __hfma2(__hsub2(*reinterpret_cast<const half2*>(&lo), one), s, l);
+            const half2 y = __hfma2(__hfma2(*reinterpret_cast<const half2*>(&hi), sixteenth, off), s, l);
+            h[2 * k] = *reinterpret_cast<const uint32_t*>(&x);
+            h[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&y);
         }
-        y[i] = *reinterpret_cast<const uint4*>(h);
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (turn ^ (uint32_t)(i << 4))), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
     }
 }
-// The same to the four 16-byte pieces of a tile's row from `piece` on.
-__device__ __forceinline__ void unpack32(uint8_t* tile, int row, int piece, const uint4& code, half2 par)
-{
-    uint8_t* dst = tile + (piece >> 3) * kBlock + row * 128;
-    uint4 y[4];
-    expand32(code, par, y);
-#pragma unroll
-    for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(dst + ((((piece & 7) + i) ^ (row & 7)) << 4)) = y[i];
-}
 
-// UNPACK: from the cache; else keys and values are FP16 rows in the workspace, copied by TMA (rows b * kv_heads + head of `cap`
-// positions each).
-template <typename T, int DIM, bool UNPACK>
+template <typename T, int DIM>
 __global__ void __launch_bounds__(kThreads, 1)
-cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out, const bool whole, const __grid_constant__ Expanded x)
+cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out, const bool whole)
 {
     using P = Prompt<DIM>;
     constexpr int kCodes = DIM / 32;                                       // 16-byte pieces of a row of codes
@@ -238,6 +205,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     __shared__ Walk::Start start;
+    __shared__ float row_scale[kRows];
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t *qs = smem, *ks = qs + kRowTiles * P::kOperand, *vs = ks + kStages * P::kOperand, *raw = vs + kStages * P::kOperand;
@@ -249,7 +217,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
     if (tid == 0) {
         for (int i = 0; i < kBars; i++) {
             const int pair = i & ~1;
-            mbar_init(bar(i), pair == kQFull || (i >= kPReady && i < kLast) ? kTile : UNPACK && (pair == kKFull || pair == kVFull) ? kUnpackThreads :
+            mbar_init(bar(i), pair == kQFull || (i >= kPReady && i < kLast) ? kTile : pair == kKFull || pair == kVFull ? kUnpackThreads :
                               pair == kKEmpty || pair == kVEmpty ? kRowTiles : 1);
         }
         abort_flag = 0;
@@ -346,82 +314,58 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
             __syncwarp();
             mbar_wait(bar(kLast + i), 0, &never);
         }
-    } else if (warp >= 8 && !UNPACK) {
-        if (warp == 8) {
-            // ---------------- copies of expanded keys and values ----------------
-            const bool leader = elect_one();
-            Walk w(a, whole, start);
-            uint32_t n = 0, issued[2] = {0, 0};
-            bool ok = true;
-            while (ok && w.advance()) {
-                const int row0 = (w.b * w.kv_heads + w.head) * x.cap;
-                for (int j = w.j0; ok && j < w.j1; j++, n++) {
-                    const uint32_t st = n & 1, parity = ((n >> 1) & 1) ^ 1;
-#pragma unroll
-                    for (int side = 0; side < 2; side++) {
-                        const uint32_t full = bar((side ? kVFull : kKFull) + st);
-                        if (!(ok = mbar_wait(bar((side ? kVEmpty : kKEmpty) + st), parity, abortp))) break;
-                        if (leader) {
-                            mbar_expect_tx(full, P::kOperand);
-#pragma unroll
-                            for (int c = 0; c < P::kBlocks; c++)
-                                tma_load_2d(smem_u32((side ? vs : ks) + st * P::kOperand + c * kBlock), side ? &x.v : &x.k, c * 64, row0 + j * kTile, full);
-                        }
-                        issued[side] = n + 1;
-                    }
-                }
-            }
-            if (!ok) abort_flag = 1;
-            __syncwarp();
-            // after an abort the copies still in flight must land before the shared memory goes away
-            if (*abortp)
-                for (int side = 0; side < 2; side++)
-                    for (uint32_t i = issued[side] > 2 ? issued[side] - 2 : 0; i < issued[side]; i++)
-                        mbar_wait(bar((side ? kVFull : kKFull) + (i & 1)), (i >> 1) & 1, &never);
-        }
     } else if (warp >= 8) {
         // ---------------- unpacking: 16 bytes of a position at once ----------------
         // A thread copies what it unpacks for the tile after this one (cp.async), and reads it back itself.
+        // Three warps for keys and three for values, so that neither waits for the other's stage.  Piece e is piece e / 128 of row e % 128; the
+        // rows of a thread agree in their last three bits, so what is exchanged is fixed.
         constexpr int kRounds = P::kRounds;
-        const int first = (warp < 12 ? warp - 8 : warp - 10) * 32 + lane;
+        const bool values = warp == 11 || warp > 13;
+        const int first = (values ? max(warp - 13, 0) : warp - 8) * 32 + lane;
+        const uint32_t mine = smem_u32(raw) + (values ? P::kRawSide : 0), mine_par = mine + kRounds * kUnpackThreads * 16, turn = (lane & 3) << 4;
+        const uint32_t tile0 = smem_u32(values ? vs : ks);
+        const int full = values ? kVFull : kKFull, empty = values ? kVEmpty : kKEmpty;
+        const uint8_t* codes = values ? a.c.vc : a.c.kc;
+        const half2* params = values ? a.c.vp : a.c.kp;
         Walk w(a, whole, start);
         uint32_t n = 0;
         bool ok = true;
         while (ok && w.advance()) {
-            const size_t row0 = cache_row(a.c, w.b, w.head, 0);
-            const auto load = [&](int side, int j) {
+            size_t at = cache_row(a.c, w.b, w.head, w.j0 * kTile);           // of the tile to be copied
+            const auto load = [&](int j) {
+                const int left = w.visible - j * kTile;                     // positions behind hold anything: they become 0
 #pragma unroll
                 for (int k = 0; k < kRounds; k++) {
-                    const int e = first + k * kUnpackThreads, c = e / kTile, p = j * kTile + e % kTile;
-                    const bool valid = c < kCodes && p < w.visible;         // positions behind hold anything: they become 0
-                    const size_t at = row0 + (valid ? p : 0);
-                    const uint32_t to = smem_u32(raw + side * P::kRawSide);
-                    copy_async<16>(to + (first + k * kUnpackThreads) * 16, (side ? a.c.vc : a.c.kc) + at * (DIM / 2) + (valid ? c * 16 : 0), valid);
-                    copy_async<4>(to + kRounds * kUnpackThreads * 16 + (first + k * kUnpackThreads) * 4, (side ? a.c.vp : a.c.kp) + at * P::kBlocks + (valid ? c / 2 : 0), valid);
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            load(0, w.j0);
-            load(1, w.j0);
-            for (int j = w.j0; ok && j < w.j1; j++, n++) {
-                const uint32_t st = n & 1, parity = ((n >> 1) & 1) ^ 1;
-#pragma unroll
-                for (int side = 0; side < 2; side++) {
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");    // the other side's copies are younger
-                    if (!(ok = mbar_wait(bar((side ? kVEmpty : kKEmpty) + st), parity, abortp))) break;
-                    const uint8_t* from = raw + side * P::kRawSide;
-#pragma unroll
-                    for (int k = 0; k < kRounds; k++) {
-                        const int e = first + k * kUnpackThreads, c = e / kTile;
-                        if (c < kCodes)
-                            unpack32((side ? vs : ks) + st * P::kOperand, e % kTile, c * 4, reinterpret_cast<const uint4*>(from)[e],
-                                     reinterpret_cast<const half2*>(from + kRounds * kUnpackThreads * 16)[e]);
+                    const int e = first + k * kUnpackThreads, c = e / kTile, row = e % kTile;
+                    if (k < kRounds - 1 || e < kCodes * kTile) {
+                        const bool valid = row < left;
+                        const size_t from = at + (valid ? row : 0);
+                        copy_async<16>(mine + e * 16, codes + from * (DIM / 2) + c * 16, valid);
+                        copy_async<4>(mine_par + e * 4, params + from * P::kBlocks + c / 2, valid);
                     }
-                    fence_async();
-                    mbar_arrive(bar((side ? kVFull : kKFull) + st));
-                    if (j + 1 < w.j1) load(side, j + 1);
-                    else asm volatile("cp.async.commit_group;" ::: "memory");
                 }
+                at += kTile;
+            };
+            load(w.j0);
+            for (int j = w.j0; j < w.j1; j++, n++) {
+                const uint32_t st = n & 1;
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                if (!(ok = mbar_wait(bar(empty + st), ((n >> 1) & 1) ^ 1, abortp))) break;
+                const uint32_t to = tile0 + st * P::kOperand;
+#pragma unroll
+                for (int k = 0; k < kRounds; k++) {
+                    const int e = first + k * kUnpackThreads, c = e / kTile;
+                    if (k < kRounds - 1 || e < kCodes * kTile) {
+                        uint4 code;
+                        uint32_t par;
+                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(code.x), "=r"(code.y), "=r"(code.z), "=r"(code.w) : "r"(mine + e * 16) : "memory");
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(par) : "r"(mine_par + e * 4) : "memory");
+                        unpack32(to + (c >> 1) * kBlock + e % kTile * 128 + (((c & 1) ^ (lane >> 2 & 1)) << 6), turn, code, *reinterpret_cast<const half2*>(&par));
+                    }
+                }
+                fence_async();
+                mbar_arrive(bar(full + st));
+                if (j + 1 < w.j1) load(j + 1);
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         }
@@ -440,44 +384,48 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
             const bool there = row < tile_rows;
             const int token = there ? r / w.per : 0, head = w.head * w.per + (there ? r % w.per : 0);
             const int sees = there ? w.span.position(token) + 1 : 0, least = w.span.position((r - row) / w.per) + 1;
-            // ---- the row of queries, with the sign of the scale ----
-            float scale2 = fabsf(a.scale) * kLog2e;
-            {
-                const uint4* src = reinterpret_cast<const uint4*>(q.p + (size_t)(w.span.row0 + token) * q.ld + (size_t)head * DIM);
-                uint4 v[DIM / 8];
-#pragma unroll
-                for (int c = 0; c < DIM / 8; c++) v[c] = there ? src[c] : make_uint4(0, 0, 0, 0);
-                float up = a.scale < 0.f ? -1.f : 1.f;
-                if constexpr (!std::is_same<T, half>::value) {
-                    float top = 0.f;
-#pragma unroll
-                    for (int c = 0; c < DIM / 8; c++)
-#pragma unroll
-                        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(as_float(reinterpret_cast<const T*>(&v[c])[e])));
-                    const int e = (__float_as_int(top) >> 23) - 127;
-                    if (top > 0.f && e < 128) {
-                        const int sh = min(14 - e, 126);
-                        up *= __int_as_float((127 + sh) << 23);
-                        scale2 *= __int_as_float((127 - sh) << 23);
-                    }
-#pragma unroll
-                    for (int c = 0; c < DIM / 8; c++) {
-                        half2 h[4];
-#pragma unroll
-                        for (int e2 = 0; e2 < 4; e2++)
-                            h[e2] = __floats2half2_rn(as_float(reinterpret_cast<const T*>(&v[c])[2 * e2]) * up, as_float(reinterpret_cast<const T*>(&v[c])[2 * e2 + 1]) * up);
-                        v[c] = *reinterpret_cast<const uint4*>(h);
-                    }
-                } else if (up < 0.f) {
-#pragma unroll
-                    for (int c = 0; c < DIM / 8; c++) v[c] = make_uint4(v[c].x ^ 0x80008000u, v[c].y ^ 0x80008000u, v[c].z ^ 0x80008000u, v[c].w ^ 0x80008000u);
-                }
-#pragma unroll
-                for (int c = 0; c < DIM / 8; c++)
-                    *reinterpret_cast<uint4*>(qs + i * P::kOperand + (c >> 3) * kBlock + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v[c];
-                fence_async();
-                mbar_arrive(bar(kQFull + i));
+            // ---- the warp's rows of queries, with the sign of the scale: kLanes lanes take a row, whole sectors at a time ----
+            constexpr int kLanes = DIM / 8, kAtOnce = 32 / kLanes;
+            const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+            const auto piece = [&](int k) {
+                const int at = (warp & 3) * 32 + k * kAtOnce + lane / kLanes;
+                return qs + i * P::kOperand + (lane % kLanes >> 3) * kBlock + at * 128 + (((lane & 7) ^ (at & 7)) << 4);
+            };
+#pragma unroll 2
+            for (int k = 0; k < 32 / kAtOnce; k++) {
+                const int at = (warp & 3) * 32 + k * kAtOnce + lane / kLanes;
+                const unsigned from = w.tile * kRows + i * kTile + (at < tile_rows ? at : 0), tok = from / (unsigned)w.per;
+                const T* src = q.p + (size_t)(w.span.row0 + tok) * q.ld + (size_t)(w.head * w.per + from - tok * w.per) * DIM + lane % kLanes * 8;
+                copy_async<16>(smem_u32(piece(k)), src, at < tile_rows);
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (!std::is_same<T, half>::value || sign) {
+                // a lane changes what it copied.  BF16 numbers become FP16 ones times a power of two of their row, the largest from 2^14 on:
+                // their exponents order the sizes
+#pragma unroll 4
+                for (int k = 0; k < 32 / kAtOnce; k++) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(piece(k));
+                    uint32_t x[4] = {v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign};
+                    if constexpr (!std::is_same<T, half>::value) {
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) top = max(top, max(x[e] & 0x7f80u, x[e] >> 16 & 0x7f80u));
+#pragma unroll
+                        for (int d = 1; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const int exponent = (int)(top >> 7) - 127, sh = exponent == 128 || top == 0 ? 0 : min(14 - exponent, 126);
+                        const float up = __int_as_float((127 + sh) << 23);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[e] = Pair2<half>::of(__uint_as_float(x[e] << 16) * up, __uint_as_float(x[e] & 0xffff0000u) * up);
+                        if (lane % kLanes == 0) row_scale[i * kTile + (warp & 3) * 32 + k * kAtOnce + lane / kLanes] = __int_as_float((127 - sh) << 23);
+                    }
+                    *reinterpret_cast<uint4*>(piece(k)) = make_uint4(x[0], x[1], x[2], x[3]);
+                }
+            }
+            fence_async();
+            __syncwarp();
+            mbar_arrive(bar(kQFull + i));
+            float scale2 = fabsf(a.scale) * kLog2e;
+            if constexpr (!std::is_same<T, half>::value) scale2 *= row_scale[i * kTile + row];
             scale2 = fmaxf(scale2, 1e-37f);                                 // a masked score times it stays -infinity
             const f32x2 scale = pair_f32(scale2, scale2);
             float m = -INFINITY, l = 0.f;
@@ -488,6 +436,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
                 ok = __all_sync(0xffffffffu, mbar_wait(bar(kSFull + u), parity, abortp));
                 if (!ok) break;
                 fence_after();
+                bool again = false;
                 uint32_t s[2][32];
                 tmem_ld32(at_s, s[0]);
                 tmem_ld32(at_s + 32, s[1]);
@@ -498,36 +447,37 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
                     for (int k = 0; k < kHalf; k++)
                         if (k >= seen) s[k / 32][k % 32] = 0xff800000u;
                 }
-                // With the maximum so far, which rarely has to move: the search for it runs beside the exponentials, and a second pass follows
-                // where it moved.
+                // With the maximum so far.  It is looked for only where the sum of the half's weights shows that one may exceed 2^kSlack, and for
+                // the first half; a second pass follows.
                 f32x2 sum[2];
                 uint32_t pw[32];
 #pragma unroll 1
-                for (int pass = 0; pass < 2; pass++) {
-                    const float ref = kLift - (m == -INFINITY ? 0.f : m);
-                    const f32x2 off = pair_f32(ref, ref);
-                    float top[2] = {-INFINITY, -INFINITY};
-                    sum[0] = sum[1] = 0ull;
+                for (bool first = j == 2 * w.j0;; first = false) {
+                    float total = INFINITY;
+                    if (!first) {
+                        const float ref = kLift - (m == -INFINITY ? 0.f : m);
+                        const f32x2 off = pair_f32(ref, ref);
+                        sum[0] = sum[1] = 0ull;
 #pragma unroll
-                    for (int k = 0; k < 32; k++) {
-                        const uint32_t(&v)[32] = s[k / 16];
-                        const uint32_t v0 = v[k % 16 * 2], v1 = v[k % 16 * 2 + 1];
-                        const f32x2 e = fma_pairs(pair_f32(v0, v1), scale, off);
-                        f32x2 w;
-                        if (k % kEvery < kPolynomial) {
-                            w = exp2_pair(e);
-                        } else {
-                            const float2 x = split_f32(e);
-                            w = pair_f32(exp2_neg(x.x), exp2_neg(x.y));
+                        for (int k = 0; k < 32; k++) {
+                            const uint32_t(&v)[32] = s[k / 16];
+                            const float2 e = split_f32(fma_pairs(pair_f32(v[k % 16 * 2], v[k % 16 * 2 + 1]), scale, off));
+                            const float x = exp2_neg(e.x), y = exp2_neg(e.y);
+                            sum[k & 1] = add_pair(sum[k & 1], pair_f32(x, y));
+                            pw[k] = Pair2<half>::of(x, y);
                         }
-                        sum[k & 1] = add_pair(sum[k & 1], w);
-                        const float2 y = split_f32(w);
-                        pw[k] = Pair2<half>::of(y.x, y.y);
-                        top[k & 1] = max3(top[k & 1], __uint_as_float(v0), __uint_as_float(v1));
+                        total = sum_pair(add_pair(sum[0], sum[1]));
                     }
+                    if (again || !__any_sync(0xffffffffu, !(total <= kMost))) {
+                        l += total;
+                        break;
+                    }
+                    again = true;
+                    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int k = 0; k < 32; k++) top[k & 1] = max3(top[k & 1], __uint_as_float(s[k / 16][k % 16 * 2]), __uint_as_float(s[k / 16][k % 16 * 2 + 1]));
                     const float mx = max3(top[0], top[0], top[1]) * scale2;
-                    if (pass || !__any_sync(0xffffffffu, !(mx <= m + kSlack))) break;
-                    const bool grows = mx > m + kSlack;
+                    const bool grows = !(total <= kMost) && mx > m;         // a row's result does not depend on the others' of its warp
                     const float f = grows ? exp2_neg(m - mx) : 1.f;         // 0 where nothing was seen before
                     if (grows) {
                         m = mx;
@@ -552,7 +502,6 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
                 }
                 if (!ok) break;
                 tmem_st32(at_s, pw);
-                l += sum_pair(add_pair(sum[0], sum[1]));
                 wait_st();
                 fence_before();
                 mbar_arrive(bar(kPReady + u));
@@ -607,78 +556,20 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
     }
 }
 
-// Rows of keys and values of the sequences of a call as FP16, rounded once; zeros up to the end of a tile of positions.
-template <int DIM>
-__global__ void __launch_bounds__(256)
-cache4_expand_kernel(const Cache4Call a, uint8_t* k, uint8_t* v, const int cap)
-{
-    pdl_launch_dependents();
-    pdl_wait();
-    const int b = blockIdx.z, g = blockIdx.y;
-    const Span sp = span_of(a.s, b, blockIdx.x == 0 && g == 0 && threadIdx.x == 0);
-    const int end = sp.n > 0 ? min((sp.len + kTile - 1) / kTile * kTile, cap) : 0;
-    constexpr int kPieces = DIM / 32, kPositions = 256 / kPieces;          // 16 bytes of codes a thread, of keys and of values
-    const int c = threadIdx.x % kPieces;
-    for (int p = blockIdx.x * kPositions + threadIdx.x / kPieces; p < end; p += gridDim.x * kPositions) {
-        const size_t row = cache_row(a.c, b, g, min(p, sp.len - 1)), to = ((size_t)(b * a.c.kv_heads + g) * cap + p) * DIM * 2 + c * 64;
-#pragma unroll
-        for (int side = 0; side < 2; side++) {
-            uint4 code = make_uint4(0, 0, 0, 0);
-            half2 par = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-            if (p < sp.len) {
-                code = reinterpret_cast<const uint4*>((side ? a.c.vc : a.c.kc) + row * (DIM / 2))[c];
-                par = (side ? a.c.vp : a.c.kp)[row * (DIM / 64) + c / 2];
-            }
-            uint4 y[4];
-            expand32(code, par, y);
-#pragma unroll
-            for (int i = 0; i < 4; i++) reinterpret_cast<uint4*>((side ? v : k) + to)[i] = y[i];
-        }
-    }
-}
-
-int encode(CUtensorMap* map, const uint8_t* p, int dim, size_t rows)
-{
-    const EncodeTiledFn enc = encode_fn();
-    if (!enc) return fail(TLLM_ERR_LAUNCH, "cuTensorMapEncodeTiled is not available from this driver");
-    const cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)dim * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)kTile}, estr[2] = {1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<uint8_t*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? TLLM_OK : fail(TLLM_ERR_LAUNCH, "cache4_prompt: cuTensorMapEncodeTiled failed with %d", (int)r);
-}
-
-template <typename T, int DIM, bool UNPACK>
-int launch_form(const Cache4Call& a, Rows<const T> q, Rows<T> out, const PromptPlan& p, cudaStream_t stream)
+template <typename T, int DIM>
+int launch(const Cache4Call& a, Rows<const T> q, Rows<T> out, const PromptPlan& p, cudaStream_t stream)
 {
     static bool attr[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return fail(TLLM_ERR_LAUNCH, "cache4_prompt: no current device");
-    const auto kernel = cache4_prompt_kernel<T, DIM, UNPACK>;
+    const auto kernel = cache4_prompt_kernel<T, DIM>;
     if (!attr[dev]) {
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<DIM>::kSmem);
         attr[dev] = true;
     }
-    Expanded x = {};
-    int st;
-    if (!UNPACK) {
-        const size_t rows = (size_t)a.c.batch * a.c.kv_heads * p.cap;
-        uint8_t *k = static_cast<uint8_t*>(a.ws) + p.join_bytes, *v = k + rows * DIM * 2;
-        x.cap = p.cap;
-        if ((st = encode(&x.k, k, DIM, rows)) || (st = encode(&x.v, v, DIM, rows))) return st;
-        const int positions = 256 / (DIM / 32), blocks = (p.cap + positions - 1) / positions;
-        st = launch_pdl("cache4_expand", cache4_expand_kernel<DIM>, dim3(blocks < 1024 ? blocks : 1024, a.c.kv_heads, a.c.batch), dim3(256), 0, stream, a, k, v, p.cap);
-        if (st) return st;
-    }
-    st = launch_pdl("cache4_prompt", kernel, dim3(p.ctas), dim3(kThreads), Prompt<DIM>::kSmem, stream, a, q, out, p.whole, x);
+    const int st = launch_pdl("cache4_prompt", kernel, dim3(p.ctas), dim3(kThreads), Prompt<DIM>::kSmem, stream, a, q, out, p.whole);
     return st || p.whole ? st : launch_cache4_join<T>(a, out, kRows, p.ctas, stream);
-}
-
-template <typename T, int DIM>
-int launch(const Cache4Call& a, Rows<const T> q, Rows<T> out, const PromptPlan& p, cudaStream_t stream)
-{
-    return p.cap ? launch_form<T, DIM, false>(a, q, out, p, stream) : launch_form<T, DIM, true>(a, q, out, p, stream);
 }
 
 }  // namespace
@@ -693,10 +584,7 @@ PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int 
     const long long grid = tiles * pairs < (1 << 20) ? tiles * pairs : (1 << 20) / pairs * pairs;
     p.whole = all >= 222;
     p.ctas = p.whole ? (int)(grid < pairs ? pairs : grid) : 148;
-    p.join_bytes = p.whole ? 0 : (join_bytes(c.dim, kRows, p.ctas) + 255) / 256 * 256;
-    const int len = max_len > 0 && max_len < c.rows ? max_len : c.rows;
-    p.cap = tiles >= 3 && pairs * len < (1 << 30) ? (len + kTile - 1) / kTile * kTile : 0;
-    p.bytes = p.join_bytes + (size_t)pairs * p.cap * c.dim * 4;
+    p.bytes = p.whole ? 0 : join_bytes(c.dim, kRows, p.ctas);
     return p;
 }
 

@@ -1,11 +1,11 @@
 // Rows of the 4-bit key/value cache: append (rotation of queries and keys, rounding of keys and values to
 // 4 bits) and read back.
 //
-// A warp has a row of a head.  Of 64 values x, limited to +-61440: l = half(min x), s = half((max x - l) / 15),
-// c = rint((x - l) / s) within 0..15; the limit keeps s c + l inside FP16.  Both differences and quotients are
-// single FP32 operations, so the codes follow from the rounded activations alone.
-#include <cfloat>
-
+// Of 64 values x, limited to +-61440: l = half(min x), s = half((max x - l) / 15), c = rint((x - l) / s) within
+// 0..15; the limit keeps s c + l inside FP16.  Both differences and quotients are single FP32 operations, so the codes
+// follow from the rounded activations alone.  Eight lanes have a group, a lane eight neighbouring values: 16 bytes in,
+// a word of codes out.  The keys and values of a head of a row stay with the same lanes, which mark a NaN in either.
+// Bound by the bytes for many rows, by the chain of loads (sequence, position, angles, row) for a few.
 #include "cache4.cuh"
 #include "launch.cuh"
 
@@ -13,7 +13,7 @@ namespace tllm {
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kThreads = 256;
 
 template <typename T>
 struct AppendArgs {
@@ -25,127 +25,263 @@ struct AppendArgs {
     Rows<T> q_out;
 };
 
-// Entries 64 g + 2 lane and the next of a row, turned.
-template <typename T, int DIM>
-__device__ __forceinline__ void turned_row(const Rotary& r, const T* x, int position, int lane, float (&y)[DIM / 32])
+// Where rows row0 .. of a CTA belong: sequence (-1: none) and position.
+template <int ROWS>
+struct Places {
+    int seq[ROWS], position[ROWS];
+};
+template <int ROWS>
+__device__ __forceinline__ void find_places(const Seqs& s, int row0, Places<ROWS>& p)
 {
-#pragma unroll
-    for (int i = 0; i < DIM / 32; i++) {
-        const int e = (i >> 1) * 64 + 2 * lane + (i & 1);
-        y[i] = as_float(x[e]);
-        if (r.turns && e < r.rot) {
-            const int pairs = r.rot / 2, pair = r.half_layout ? e % pairs : e >> 1;
-            const bool second = r.half_layout ? e >= pairs : e & 1;
-            const float other = as_float(x[r.half_layout ? (second ? e - pairs : e + pairs) : e ^ 1]);
-            float c, s;
-            turn(r, r.turns[pair], position, c, s);
-            y[i] = as_float(as_type<T>(second ? y[i] * c + other * s : y[i] * c - other * s));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = row0 + warp;
+    if (warp < ROWS) {
+        // the first sequence whose end lies behind the row; 32 at once, all their numbers in one round of loads
+        int seq = -1, position = 0;
+        for (int b0 = 0; b0 < s.batch && row < s.tokens; b0 += 32) {
+            const int b = b0 + lane;
+            Span sp;
+            sp.row0 = sp.n = sp.len = 0;
+            int end = 0;
+            if (b < s.batch) {
+                end = s.first[b + 1];
+                sp = span_of(s, b, false);
+            }
+            const uint32_t m = __ballot_sync(0xffffffffu, b < s.batch && row < end);
+            if (!m) continue;
+            const int from = __ffs(m) - 1, start = __shfl_sync(0xffffffffu, sp.row0, from), n = __shfl_sync(0xffffffffu, sp.n, from);
+            position = __shfl_sync(0xffffffffu, sp.len, from) - n + row - start;
+            if (row >= start && row - start < n) seq = b0 + from;
+            break;
+        }
+        if (lane == 0) {
+            p.seq[warp] = seq;
+            p.position[warp] = position;
         }
     }
+    if (row0 == 0 && blockIdx.y == 0 && warp == kThreads / 32 - 1)
+        for (int b = lane; b < s.batch; b += 32) span_of(s, b, true);
 }
 
-// Writes a row of DIM values; `bad`: its params become NaN.
-template <int DIM>
-__device__ __forceinline__ void write_row(uint8_t* codes, half2* params, size_t row, int lane, const float (&x)[DIM / 32], bool bad)
+// Sign-exact comparisons of eight lanes.
+__device__ __forceinline__ float max8(float v)
 {
 #pragma unroll
-    for (int g = 0; g < DIM / 64; g++) {
-        float v[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const float a = x[2 * g + i];
-            v[i] = a != a ? 0.f : fminf(fmaxf(a, -TLLM_CACHE4_LIMIT), TLLM_CACHE4_LIMIT);
-        }
-        const half l = __float2half_rn(-warp_max(fmaxf(-v[0], -v[1])));
-        const float lf = __half2float(l);
-        const half s = __float2half_rn((warp_max(fmaxf(v[0], v[1])) - lf) / 15.f);
-        const float sf = __half2float(s);
-        uint32_t word = 0;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const float c = sf > 0.f ? fminf(fmaxf(rintf((v[i] - lf) / sf), 0.f), 15.f) : 0.f;
-            word |= (uint32_t)c << (4 * (lane & 3) + 16 * i);
-        }
-        word |= __shfl_xor_sync(0xffffffffu, word, 1);
-        word |= __shfl_xor_sync(0xffffffffu, word, 2);
-        if ((lane & 3) == 0) reinterpret_cast<uint32_t*>(codes + row * (DIM / 2))[g * 8 + (lane >> 2)] = word;
-        if (lane == 0) params[row * (DIM / 64) + g] = bad ? __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff)) : __halves2half2(s, l);
-    }
+    for (int o = 1; o < 8; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
 }
 
-// Warps of a row: one for each query head, one for each key/value head.
-template <typename T, int DIM>
+// The codes and (s, l) of the group that eight lanes hold.
+__device__ __forceinline__ void write_group(uint8_t* codes, half2* params, size_t row, int words, int lane_of_row, const float (&x)[8], bool bad, bool write)
+{
+    float v[8], low = INFINITY, high = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        v[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -TLLM_CACHE4_LIMIT), TLLM_CACHE4_LIMIT);
+        low = fminf(low, v[i]);
+        high = fmaxf(high, v[i]);
+    }
+    const half l = __float2half_rn(-max8(-low));
+    const float lf = __half2float(l);
+    const half s = __float2half_rn((max8(high) - lf) / 15.f);
+    const float sf = __half2float(s);
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float c = sf > 0.f ? fminf(fmaxf(rintf((v[i] - lf) / sf), 0.f), 15.f) : 0.f;
+        word |= (uint32_t)c << (4 * (i >> 1) + 16 * (i & 1));
+    }
+    if (!write) return;
+    reinterpret_cast<uint32_t*>(codes)[row * words + lane_of_row] = word;
+    if ((lane_of_row & 7) == 0)
+        params[row * (words / 8) + lane_of_row / 8] = bad ? __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff)) : __halves2half2(s, l);
+}
+
+// blockIdx.y = 0: keys and values, 1: queries.
+template <typename T, int DIM, int ROWS>
 __global__ void __launch_bounds__(kThreads)
 cache4_append_kernel(const AppendArgs<T> a)
 {
+    __shared__ Places<ROWS> at;
+    __shared__ float2 cs[ROWS][DIM / 2];
     pdl_launch_dependents();
-    pdl_wait();
-    const int lane = threadIdx.x & 31, row = blockIdx.x, h = blockIdx.y * kWarps + (threadIdx.x >> 5);
-    if (h >= a.heads + a.c.kv_heads) return;
-    if (row == 0 && h == 0)
-        for (int b = lane; b < a.s.batch; b += 32) span_of(a.s, b, true);
-    const int b = seq_of_row(a.s, row, lane);
-    if (b >= a.s.batch) return;
-    const Span sp = span_of(a.s, b, false);
-    const int position = sp.position(row - sp.row0);
-    if (position < 0 || row < sp.row0) return;
-    float y[DIM / 32];
-    if (h < a.heads) {
-        turned_row<T, DIM>(a.r, a.q.p + (size_t)row * a.q.ld + (size_t)h * DIM, position, lane, y);
-        __syncwarp();                                       // q_out may be q
-        T* o = a.q_out.p + (size_t)row * a.q_out.ld + (size_t)h * DIM;
+    const int tid = threadIdx.x, row0 = blockIdx.x * ROWS;
+    const int pairs = a.r.turns ? a.r.rot / 2 : 0, rows = min(ROWS, a.s.tokens - row0);
+    const bool whole = !a.r.half_layout || pairs % 8 == 0;
+    const Turn<T> t(a.r, DIM);
+    constexpr int kLanes = DIM / 8;                        // of a row of a head
+    const int lane = tid % kLanes, e0 = lane * 8;
+    int h = tid / t.per_head, u = tid % t.per_head;
+    uint4 w[ROWS][2];
+    const auto load = [&] {
 #pragma unroll
-        for (int i = 0; i < DIM / 32; i++) o[(i >> 1) * 64 + 2 * lane + (i & 1)] = as_type<T>(y[i]);
+        for (int r = 0; r < ROWS; r++)
+            if (r < rows) t.load(a.q.p + (size_t)(row0 + r) * a.q.ld + (size_t)h * DIM, u, w[r]);
+    };
+    uint4 kv[3];                                           // key, value, what turns with the key
+    const auto load_kv = [&](int i) {
+        const int g = i % a.c.kv_heads, r = i / a.c.kv_heads;
+        if (r >= rows) return;
+        const T* x = a.k.p + (size_t)(row0 + r) * a.k.ld + (size_t)g * DIM;
+        kv[0] = *reinterpret_cast<const uint4*>(x + e0);
+        kv[1] = *reinterpret_cast<const uint4*>(a.v.p + (size_t)(row0 + r) * a.v.ld + (size_t)g * DIM + e0);
+        if (a.r.half_layout && whole && e0 < 2 * pairs) kv[2] = *reinterpret_cast<const uint4*>(x + (e0 >= pairs ? e0 - pairs : e0 + pairs));
+    };
+    pdl_wait();
+    // the rows are on their way while their places and angles are found
+    const bool queries = blockIdx.y == 1;
+    if (!queries) load_kv(tid / kLanes);
+    else if (whole && h < a.heads) load();
+    find_places<ROWS>(a.s, row0, at);
+    __syncthreads();
+    for (int i = tid; i < ROWS * pairs; i += kThreads) {
+        const int r = i / pairs, p = i % pairs;
+        turn(a.r, a.r.turns[p], at.position[r], cs[r][p].x, cs[r][p].y);
+    }
+    __syncthreads();
+    if (queries) {
+        if (whole) {
+            const int step_h = kThreads / t.per_head, step_u = kThreads % t.per_head;
+            for (bool again = false; h < a.heads; again = true) {
+                if (again) load();
+#pragma unroll
+                for (int r = 0; r < ROWS; r++)
+                    if (r < rows && at.seq[r] >= 0 && at.position[r] >= 0)
+                        t.turn_and_store(a.q_out.p + (size_t)(row0 + r) * a.q_out.ld + (size_t)h * DIM, u, w[r], cs[r]);
+                h += step_h;
+                u += step_u;
+                if (u >= t.per_head) {
+                    u -= t.per_head;
+                    h++;
+                }
+            }
+            return;
+        }
+        const int per_head = DIM - pairs;
+        for (int i = tid; i < ROWS * a.heads * per_head; i += kThreads) {
+            const int e = i % per_head, h = i / per_head % a.heads, r = i / per_head / a.heads;
+            if (at.seq[r] < 0 || at.position[r] < 0) continue;
+            const T* x = a.q.p + (size_t)(row0 + r) * a.q.ld + (size_t)h * DIM;
+            T* y = a.q_out.p + (size_t)(row0 + r) * a.q_out.ld + (size_t)h * DIM;
+            if (e >= pairs) {
+                y[e + pairs] = x[e + pairs];
+                continue;
+            }
+            const float2 c = cs[r][e];
+            const float x1 = as_float(x[e]), x2 = as_float(x[e + pairs]);
+            y[e] = as_type<T>(turned_first(x1, x2, c));
+            y[e + pairs] = as_type<T>(turned_second(x1, x2, c));
+        }
         return;
     }
-    const int g = h - a.heads;
-    const size_t at = cache_row(a.c, b, g, position);
-    float v[DIM / 32];
-    turned_row<T, DIM>(a.r, a.k.p + (size_t)row * a.k.ld + (size_t)g * DIM, position, lane, y);
-    bool bad = false;
+    // all lanes of a warp stay together: those without a row write nothing
+    for (int i0 = 0; i0 < ROWS * a.c.kv_heads; i0 += kThreads / kLanes) {
+        const int i = i0 + tid / kLanes, g = i % a.c.kv_heads, r = i / a.c.kv_heads;
+        const bool write = r < rows && at.seq[r] >= 0 && at.position[r] >= 0;
+        if (i0 > 0) load_kv(i);
+        Vec<T> k, v;
+        const T* x = a.k.p + (size_t)(row0 + (write ? r : 0)) * a.k.ld + (size_t)g * DIM;
+        if (write) {
+            k.load(reinterpret_cast<const T*>(&kv[0]));
+            v.load(reinterpret_cast<const T*>(&kv[1]));
+            if (e0 < 2 * pairs) {
+                if (!a.r.half_layout) {
 #pragma unroll
-    for (int i = 0; i < DIM / 32; i++) {
-        v[i] = as_float(a.v.p[(size_t)row * a.v.ld + (size_t)g * DIM + (i >> 1) * 64 + 2 * lane + (i & 1)]);
-        bad = bad || y[i] != y[i] || v[i] != v[i];
+                    for (int e = 0; e < 8; e += 2)
+                        if (e0 + e < 2 * pairs) {
+                            const float2 c = cs[r][(e0 + e) / 2];
+                            const float x1 = k.v[e], x2 = k.v[e + 1];
+                            k.v[e] = as_float(as_type<T>(turned_first(x1, x2, c)));
+                            k.v[e + 1] = as_float(as_type<T>(turned_second(x1, x2, c)));
+                        }
+                } else if (whole) {
+                    const bool second = e0 >= pairs;
+                    Vec<T> o;
+                    o.load(reinterpret_cast<const T*>(&kv[2]));
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float2 c = cs[r][(second ? e0 - pairs : e0) + e];
+                        k.v[e] = as_float(as_type<T>(second ? turned_second(o.v[e], k.v[e], c) : turned_first(k.v[e], o.v[e], c)));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (e0 + e < 2 * pairs) {
+                            const bool second = e0 + e >= pairs;
+                            const float2 c = cs[r][second ? e0 + e - pairs : e0 + e];
+                            const float o = as_float(x[second ? e0 + e - pairs : e0 + e + pairs]);
+                            k.v[e] = as_float(as_type<T>(second ? turned_second(o, k.v[e], c) : turned_first(k.v[e], o, c)));
+                        }
+                }
+            }
+        }
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (!write) k.v[e] = v.v[e] = 0.f;
+            bad = bad || k.v[e] != k.v[e] || v.v[e] != v.v[e];
+        }
+        bad = __ballot_sync(0xffffffffu, bad) >> ((tid & 31) / kLanes * kLanes) & (kLanes == 32 ? 0xffffffffu : (1u << kLanes) - 1);
+        const size_t to = write ? cache_row(a.c, at.seq[r], g, at.position[r]) : 0;
+        write_group(a.c.kc, a.c.kp, to, DIM / 8, lane, k.v, bad, write);
+        write_group(a.c.vc, a.c.vp, to, DIM / 8, lane, v.v, false, write);
     }
-    bad = __any_sync(0xffffffffu, bad);
-    write_row<DIM>(a.c.kc, a.c.kp, at, lane, y, bad);
-    write_row<DIM>(a.c.vc, a.c.vp, at, lane, v, false);
 }
 
-template <typename T, int DIM>
+// A word of codes a thread, eight values.
+template <typename T, int DIM, int ROWS>
 __global__ void __launch_bounds__(kThreads)
 cache4_read_kernel(const Cache4 c, const Seqs s, const Rows<T> k, const Rows<T> v)
 {
+    __shared__ Places<ROWS> at;
     pdl_launch_dependents();
+    const int row0 = blockIdx.x * ROWS;
     pdl_wait();
-    const int lane = threadIdx.x & 31, row = blockIdx.x, g = blockIdx.y * kWarps + (threadIdx.x >> 5);
-    if (g >= c.kv_heads) return;
-    if (row == 0 && g == 0)
-        for (int b = lane; b < s.batch; b += 32) span_of(s, b, true);
-    const int b = seq_of_row(s, row, lane);
-    if (b >= s.batch) return;
-    const Span sp = span_of(s, b, false);
-    const int position = sp.position(row - sp.row0);
-    if (row < sp.row0) return;
-    const size_t at = cache_row(c, b, g, max(position, 0));
+    find_places<ROWS>(s, row0, at);
+    __syncthreads();
+    constexpr int kWords = DIM / 8;
+    for (int i = threadIdx.x; i < ROWS * c.kv_heads * kWords; i += kThreads) {
+        const int word = i % kWords, g = i / kWords % c.kv_heads, r = i / kWords / c.kv_heads;
+        if (at.seq[r] < 0) continue;
+        const bool held = at.position[r] >= 0;
+        const size_t row = held ? cache_row(c, at.seq[r], g, at.position[r]) : 0;
 #pragma unroll
-    for (int side = 0; side < 2; side++) {
-        const Rows<T>& o = side ? v : k;
-        if (!o.p) continue;
+        for (int side = 0; side < 2; side++) {
+            const Rows<T>& o = side ? v : k;
+            if (!o.p) continue;
+            const uint32_t w = held ? reinterpret_cast<const uint32_t*>(side ? c.vc : c.kc)[row * kWords + word] : 0;
+            const float2 p = held ? __half22float2((side ? c.vp : c.kp)[row * (DIM / 64) + word / 8]) : make_float2(0.f, 0.f);
+            T* y = o.p + (size_t)(row0 + r) * o.ld + (size_t)g * DIM + word * 8;
 #pragma unroll
-        for (int i = 0; i < DIM / 64; i++) {
-            float2 x = make_float2(0.f, 0.f);
-            if (position >= 0) {
-                const uint32_t w = reinterpret_cast<const uint32_t*>((side ? c.vc : c.kc) + at * (DIM / 2))[i * 8 + (lane >> 2)] >> (4 * (lane & 3));
-                const float2 p = __half22float2((side ? c.vp : c.kp)[at * (DIM / 64) + i]);
-                x = make_float2(fmaf((float)(w & 15), p.x, p.y), fmaf((float)((w >> 16) & 15), p.x, p.y));
+            for (int h = 0; h < 8 / Vec<T>::n; h++) {
+                Vec<T> x;
+#pragma unroll
+                for (int e = 0; e < Vec<T>::n; e++) {
+                    const int i8 = h * Vec<T>::n + e;
+                    x.v[e] = fmaf((float)((w >> (4 * (i8 >> 1) + 16 * (i8 & 1))) & 15), p.x, p.y);
+                }
+                x.store(y + h * Vec<T>::n);
             }
-            T* y = o.p + (size_t)row * o.ld + (size_t)g * DIM + i * 64 + 2 * lane;
-            y[0] = as_type<T>(x.x);
-            y[1] = as_type<T>(x.y);
         }
     }
+}
+
+constexpr int kMany = 4, kManyFrom = 4 * 148;              // rows a CTA where the CTAs still fill the SMs
+
+template <typename T, int DIM>
+int append(const AppendArgs<T>& a, cudaStream_t stream)
+{
+    const unsigned parts = a.heads > 0 ? 2 : 1;
+    if (a.s.tokens >= kManyFrom)
+        return launch_pdl("cache4_append", cache4_append_kernel<T, DIM, kMany>, dim3((a.s.tokens + kMany - 1) / kMany, parts), dim3(kThreads), 0, stream, a);
+    return launch_pdl("cache4_append", cache4_append_kernel<T, DIM, 1>, dim3(a.s.tokens, parts), dim3(kThreads), 0, stream, a);
+}
+
+template <typename T, int DIM>
+int read(const Cache4& c, const Seqs& s, Rows<T> k, Rows<T> v, cudaStream_t stream)
+{
+    if (s.tokens >= kManyFrom)
+        return launch_pdl("cache4_read", cache4_read_kernel<T, DIM, kMany>, dim3((s.tokens + kMany - 1) / kMany), dim3(kThreads), 0, stream, c, s, k, v);
+    return launch_pdl("cache4_read", cache4_read_kernel<T, DIM, 1>, dim3(s.tokens), dim3(kThreads), 0, stream, c, s, k, v);
 }
 
 }  // namespace
@@ -155,17 +291,15 @@ int launch_cache4_append(const Cache4& c, const Rotary& r, const Seqs& s, Rows<c
                          cudaStream_t stream)
 {
     if (s.tokens == 0 || s.batch == 0) return TLLM_OK;
-    const dim3 grid(s.tokens, (heads + c.kv_heads + kWarps - 1) / kWarps);
-    return launch_pdl("cache4_append", c.dim == 64 ? cache4_append_kernel<T, 64> : cache4_append_kernel<T, 128>, grid, dim3(kThreads), 0, stream,
-                      AppendArgs<T>{c, r, s, heads, q, k, v, q_out});
+    const AppendArgs<T> a = {c, r, s, heads, q, k, v, q_out};
+    return c.dim == 64 ? append<T, 64>(a, stream) : append<T, 128>(a, stream);
 }
 
 template <typename T>
 int launch_cache4_read(const Cache4& c, const Seqs& s, Rows<T> k, Rows<T> v, cudaStream_t stream)
 {
     if (s.tokens == 0 || s.batch == 0) return TLLM_OK;
-    return launch_pdl("cache4_read", c.dim == 64 ? cache4_read_kernel<T, 64> : cache4_read_kernel<T, 128>,
-                      dim3(s.tokens, (c.kv_heads + kWarps - 1) / kWarps), dim3(kThreads), 0, stream, c, s, k, v);
+    return c.dim == 64 ? read<T, 64>(c, s, k, v, stream) : read<T, 128>(c, s, k, v, stream);
 }
 
 #define TLLM_INSTANTIATE(T)                                                                                                                       \

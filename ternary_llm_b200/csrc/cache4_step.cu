@@ -108,6 +108,8 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
     pdl_wait();
 
     __shared__ typename Work<ROWS, kStepChunk>::Start start;
+    __shared__ uint32_t digits[NS * GR * 4][32];
+    __shared__ float2 worth[NS * GR][4];
     Work<ROWS, kStepChunk> work(a.s, per, a.c.kv_heads, whole);
     if (warp == 0) work.find(blockIdx.x, gridDim.x, lane, &start);
     if (!whole && tid == 0) entry_of(a.ws, blockIdx.x)->parts = 0;
@@ -166,64 +168,67 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
         for (int i = 0; i < St::kSlots - 1; i++) load(i);
 
         // ---- the query rows: digits for the first product, their sums, what a unit of a digit is worth ----
+        // A warp makes those of four rows and a group, all read them.
+        for (int k = warp; k < NS * GR; k += kWarps) {
+            const int n = k / GR, gr = k % GR, rr = St::row(n, g >> 1), r = r0 + rr;       // columns 2 i and 2 i + 1: digits of a row
+            const bool there = rr < tile_rows;
+            const T* qp = q.p + (size_t)(sp.row0 + (there ? r / per : 0)) * q.ld + (size_t)(work.head * per + (there ? r % per : 0)) * DIM + 64 * gr + 16 * t;
+            float f[2][8], top = 0.f;
+            bool odd = false;
+            uint4 v[2];
+#pragma unroll
+            for (int w = 0; w < 2; w++) v[w] = there ? reinterpret_cast<const uint4*>(qp)[w] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < 2; w++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    f[w][i] = as_float(reinterpret_cast<const T*>(&v[w])[i]);
+                    top = fmaxf(top, fabsf(f[w][i]));
+                    odd = odd || !(fabsf(f[w][i]) < INFINITY);
+                }
+#pragma unroll
+            for (int d = 1; d < 4; d <<= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                odd = __shfl_xor_sync(0xffffffffu, odd, d) || odd;
+            }
+            // sizes that a quotient of FP32 numbers can hold; smaller ones are zero in FP16 scores
+            top = fmaxf(top, 1e-30f);
+            const float by = kDigits / top;
+            int total = 0;
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                uint32_t b[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int x = odd ? 0 : __float2int_rn(f[w][i] * by), hi = (x + 128) >> 8;
+                    total += x;
+                    b[i] = (uint32_t)(g & 1 ? x - hi * 256 : hi) & 0xff;
+                }
+                // bytes as the codes lie in a word: low nibbles 0, 2, 4, 6 are entries 0, 4, 1, 5, high ones 2, 6, 3, 7
+                digits[(k * 2 + w) * 2][lane] = b[0] | b[4] << 8 | b[1] << 16 | b[5] << 24;
+                digits[(k * 2 + w) * 2 + 1][lane] = b[2] | b[6] << 8 | b[3] << 16 | b[7] << 24;
+            }
+#pragma unroll
+            for (int d = 1; d < 4; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+            // a query that is not finite has no scores
+            if (t == 0 && !(g & 1)) worth[k][g >> 1] = make_float2((float)total, odd ? NAN : top / kDigits * (a.scale * 1.4426950408889634f));
+        }
+        __syncthreads();
         uint32_t qd[NS][GR][2][2];
         float qsum[NS][GR], unit_q[NS][GR];
         int sees[NS], least = INT_MAX;
 #pragma unroll
         for (int n = 0; n < NS; n++) {
-            const int rr = St::row(n, g >> 1), r = r0 + rr;                // columns 2 i and 2 i + 1: digits of a row
-            const bool there = rr < tile_rows;
-            const T* qp = q.p + (size_t)(sp.row0 + (there ? r / per : 0)) * q.ld + (size_t)(work.head * per + (there ? r % per : 0)) * DIM;
-            float sum[GR], worth[GR];
 #pragma unroll
             for (int gr = 0; gr < GR; gr++) {
-                float f[2][8], top = 0.f;
-                bool odd = false;
+                const int k = n * GR + gr;
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (there) v = *reinterpret_cast<const uint4*>(qp + 64 * gr + 16 * t + 8 * w);
-                    const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        f[w][i] = as_float(e[i]);
-                        top = fmaxf(top, fabsf(f[w][i]));
-                        odd = odd || !(fabsf(f[w][i]) < INFINITY);
-                    }
-                }
-#pragma unroll
-                for (int d = 1; d < 4; d <<= 1) {
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    odd = __shfl_xor_sync(0xffffffffu, odd, d) || odd;
-                }
-                // sizes that a quotient of FP32 numbers can hold; smaller ones are zero in FP16 scores
-                worth[gr] = fmaxf(top, 1e-30f) / kDigits;
-                const float by = kDigits / fmaxf(top, 1e-30f);
-                int total = 0;
-#pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    uint32_t b[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int v = odd ? 0 : __float2int_rn(f[w][i] * by), hi = (v + 128) >> 8;
-                        total += v;
-                        b[i] = (uint32_t)(g & 1 ? v - hi * 256 : hi) & 0xff;
-                    }
-                    // bytes as the codes lie in a word: low nibbles 0, 2, 4, 6 are entries 0, 4, 1, 5, high ones 2, 6, 3, 7
-                    qd[n][gr][w][0] = b[0] | b[4] << 8 | b[1] << 16 | b[5] << 24;
-                    qd[n][gr][w][1] = b[2] | b[6] << 8 | b[3] << 16 | b[7] << 24;
-                }
-#pragma unroll
-                for (int d = 1; d < 4; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-                sum[gr] = (float)total;
-                if (odd) worth[gr] = NAN;                                  // a query that is not finite has no scores
+                for (int w = 0; w < 4; w++) qd[n][gr][w >> 1][w & 1] = digits[k * 4 + w][lane];
+                const float2 u = worth[k][t];
+                qsum[n][gr] = u.x;
+                unit_q[n][gr] = u.y;
             }
             const int rt = St::row(n, t);
-#pragma unroll
-            for (int gr = 0; gr < GR; gr++) {
-                qsum[n][gr] = __shfl_sync(0xffffffffu, sum[gr], 8 * t);
-                unit_q[n][gr] = __shfl_sync(0xffffffffu, worth[gr], 8 * t) * (a.scale * 1.4426950408889634f);
-            }
             sees[n] = rt < tile_rows ? sp.position((r0 + rt) / per) + 1 : 0;
             if (rt < tile_rows) least = min(least, sees[n]);
         }

@@ -39,8 +39,8 @@ int launch_cache4_step(const Cache4Call& a, Rows<const T> q, Rows<T> out, const 
 
 struct PromptPlan {
     bool whole;
-    int ctas, cap;                                   // cap: positions of a sequence that are expanded first, 0: none
-    size_t join_bytes, bytes;
+    int ctas;
+    size_t bytes;
 };
 PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int max_len);
 template <typename T>
@@ -121,10 +121,13 @@ struct Work {
     // by one warp: where part c of `parts` begins, and reports what is wrong with the sequences
     __device__ __forceinline__ void find(int c, int parts, int lane, Start* out) const
     {
-        int total = 0;
+        int total = 0, mine = 0;                      // mine: units of a head of the lane's sequence, of the last 32
+        Span sp;
         for (int b0 = 0; b0 < s.batch; b0 += 32) {
+            sp = lane_span(b0 + lane);
             if (c == 0 && b0 + lane < s.batch) span_of(s, b0 + lane, true);
-            total += __reduce_add_sync(0xffffffffu, units(lane_span(b0 + lane), lane) * kv_heads);
+            mine = units(sp, lane);
+            total += __reduce_add_sync(0xffffffffu, mine * kv_heads);
         }
         Start r;
         r.share = max((total + parts - 1) / parts, whole ? 1 : kLeast);
@@ -132,25 +135,32 @@ struct Work {
         r.to = min(r.x + r.share, total);
         r.b = r.head = r.tile = r.offset = 0;
         if (r.x < r.to) {
-            int at = r.x, u = 0;                      // u: units of a head of the sequence
+            int at = r.x, u = 0, i = 0;               // u: units of a head of the sequence
             for (int b0 = 0; b0 < s.batch; b0 += 32) {
-                const int mine = units(lane_span(b0 + lane), lane), up_to = scan(mine * kv_heads, lane);
+                if (s.batch > 32) {
+                    sp = lane_span(b0 + lane);
+                    mine = units(sp, lane);
+                }
+                const int up_to = scan(mine * kv_heads, lane);
                 const uint32_t m = __ballot_sync(0xffffffffu, up_to > at);
-                const int i = m ? __ffs(m) - 1 : 31, end = __shfl_sync(0xffffffffu, up_to, i);
+                i = m ? __ffs(m) - 1 : 31;
+                const int end = __shfl_sync(0xffffffffu, up_to, i);
                 u = __shfl_sync(0xffffffffu, mine, i);
                 at -= m ? end - u * kv_heads : end;
                 r.b = b0 + i;
                 if (m) break;
             }
-            const Span sp = span_of(s, r.b, false);
+            sp.n = __shfl_sync(0xffffffffu, sp.n, i);
+            sp.len = __shfl_sync(0xffffffffu, sp.len, i);
             r.head = at / u;
             at -= r.head * u;
             const int tiles = tiles_of(sp);
-            for (;; r.tile += 32) {
-                const int mine = r.tile + lane < tiles ? units_of(sp, r.tile + lane) : 0, up_to = scan(mine, lane);
+            for (; tiles > 1; r.tile += 32) {
+                const int of = r.tile + lane < tiles ? units_of(sp, r.tile + lane) : 0, up_to = scan(of, lane);
                 const uint32_t m = __ballot_sync(0xffffffffu, up_to > at);
-                const int i = m ? __ffs(m) - 1 : 31, end = __shfl_sync(0xffffffffu, up_to, i);
-                at -= m ? end - __shfl_sync(0xffffffffu, mine, i) : end;
+                i = m ? __ffs(m) - 1 : 31;
+                const int end = __shfl_sync(0xffffffffu, up_to, i);
+                at -= m ? end - __shfl_sync(0xffffffffu, of, i) : end;
                 if (m) {
                     r.tile += i;
                     break;

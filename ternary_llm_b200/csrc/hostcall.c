@@ -1,4 +1,4 @@
-/* The three operators on prepared weights, from Python to the C ABI in one native call.
+/* The three operators on prepared weights and those of the 4-bit cache, from Python to the C ABI in one native call.
  *
  * A call of a small projection is bound by the host: through ctypes and checks written in Python it
  * takes 9.7 us, of which 3.2 are an object for the current stream, 2.5 the checks of three tensors and 1
@@ -11,6 +11,8 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <limits.h>
+
+#include "tllm_b200_cache4.h"
 
 typedef int (*gemv_fn)(const void*, const void*, void*, int, int, int, void*);
 typedef int (*gemv_int8_fn)(const void*, const void*, float, void*, int, int, void*);
@@ -130,6 +132,207 @@ static PyObject* gemm_packed(PyObject* self, PyObject* const* a, Py_ssize_t n)
     return PyLong_FromLong(status);
 }
 
+/* ---- 4-bit cache: handles are the bytes of their C structs, made once by the Python objects that own the memory ---- */
+static int (*f_rotary)(int, const tllm_b200_rotary_table*, const int*, int, const tllm_b200_heads*, const tllm_b200_heads*, int, const tllm_b200_heads*,
+                       const tllm_b200_heads*, int, int, int, void*);
+static int (*f_append)(const tllm_b200_cache4*, int, const tllm_b200_rotary_table*, const int*, const int*, int, const tllm_b200_heads*,
+                       const tllm_b200_heads*, int, const tllm_b200_heads*, const tllm_b200_heads*, void*);
+static int (*f_read)(const tllm_b200_cache4*, int, const int*, const int*, int, const tllm_b200_heads*, const tllm_b200_heads*, void*);
+static int (*f_attention)(const tllm_b200_cache4*, int, const int*, const int*, int, const tllm_b200_heads*, const tllm_b200_heads*, int, float, int, int,
+                          void*, size_t, void*);
+static int (*f_workspace)(const tllm_b200_cache4*, int, int, int, int, size_t*);
+static PyObject *d_types[3], *d_int32;                          /* FP16, BF16, FP32 as the C ABI numbers them */
+static PyObject *s_shape, *s_stride, *s_new_empty;
+
+/* Three numbers of a tuple; consumes the reference. */
+static int triple(PyObject* o, long long* v)
+{
+    int ok = o && PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 3;
+    for (int i = 0; ok && i < 3; i++) {
+        v[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(o, i));
+        ok = !PyErr_Occurred();
+    }
+    PyErr_Clear();
+    Py_XDECREF(o);
+    return ok;
+}
+
+/* 1 and the rows of a CUDA tensor [tokens, heads, dim] whose heads lie behind one another; *type, and entries of `shape`, are set where
+ * they are -1 and must agree otherwise.  Empty tensors go the other way. */
+static int rows3(PyObject* t, long long device, int* type, long long* shape, tllm_b200_heads* r)
+{
+    long long n[3], st[3];
+    if (!is_true(PyObject_GetAttr(t, s_is_cuda))) return 0;
+    PyObject* d = PyObject_GetAttr(t, s_dtype);
+    if (!d) PyErr_Clear();
+    Py_XDECREF(d);
+    int k = 0;
+    while (k < 3 && d != d_types[k]) k++;
+    if (k == 3 || (*type >= 0 && *type != k) || number(method(t, s_get_device)) != device) return 0;
+    *type = k;
+    if (!triple(PyObject_GetAttr(t, s_shape), n) || !triple(method(t, s_stride), st)) return 0;
+    for (int i = 0; i < 3; i++) {
+        if (n[i] < 1 || n[i] > INT_MAX || (shape[i] >= 0 && shape[i] != n[i])) return 0;
+        shape[i] = n[i];
+    }
+    if ((n[2] > 1 && st[2] != 1) || (n[1] > 1 && st[1] != n[2])) return 0;
+    const long long a = number(method(t, s_data_ptr));
+    if (a <= 0) return 0;
+    r->p = (void*)a;
+    r->ld = n[0] > 1 ? st[0] : n[1] * n[2];
+    return 1;
+}
+
+/* The C struct that `o`, a bytes object made on `device`, holds. */
+static const void* handle(PyObject* o, PyObject* device, long long current, size_t size)
+{
+    if (!PyBytes_CheckExact(o) || (size_t)PyBytes_GET_SIZE(o) != size || !PyLong_CheckExact(device) || PyLong_AsLong(device) != current) return NULL;
+    return PyBytes_AS_STRING(o);
+}
+
+/* int32 tensors of batch + 1 and batch entries */
+static int sequences(const tllm_b200_cache4* c, PyObject* first, PyObject* lens, long long dev, void** f, void** n)
+{
+    return c->batch > 0 && tensor(first, d_int32, dev, (long long)c->batch + 1, f) && number(method(first, s_numel)) == (long long)c->batch + 1 &&
+           tensor(lens, d_int32, dev, c->batch, n) && number(method(lens, s_numel)) == c->batch;
+}
+
+/* a plain int of 0 .. INT_MAX, else -1 */
+static int not_negative(PyObject* o)
+{
+    if (!PyLong_CheckExact(o)) return -1;
+    int over = 0;
+    const long long v = PyLong_AsLongLongAndOverflow(o, &over);
+    return over || v < 0 || v > INT_MAX ? -1 : (int)v;
+}
+
+/* (table, its device, q, k or None, positions, q_out or None, k_out or None, inverse) */
+static PyObject* rotary(PyObject* self, PyObject* const* a, Py_ssize_t n)
+{
+    long long dev, q3[3] = {-1, -1, -1}, k3[3];
+    void *positions, *stream;
+    int type = -1;
+    tllm_b200_heads q, qo, k, ko;
+    const tllm_b200_rotary_table* t;
+    if (n != 8 || !f_rotary || !where(&dev, &stream) || !(t = handle(a[0], a[1], dev, sizeof *t)) || !rows3(a[2], dev, &type, q3, &q) ||
+        !PyBool_Check(a[7]))
+        Py_RETURN_NONE;
+    const int keys = a[3] != Py_None;
+    k3[0] = q3[0], k3[1] = -1, k3[2] = q3[2];
+    if (!rows3(a[5] == Py_None ? a[2] : a[5], dev, &type, q3, &qo) || (!keys && a[6] != Py_None) ||
+        (keys && (!rows3(a[3], dev, &type, k3, &k) || !rows3(a[6] == Py_None ? a[3] : a[6], dev, &type, k3, &ko))) ||
+        !tensor(a[4], d_int32, dev, q3[0], &positions))
+        Py_RETURN_NONE;
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = f_rotary(type, t, positions, (int)q3[0], &q, &qo, (int)q3[1], keys ? &k : NULL, keys ? &ko : NULL, keys ? (int)k3[1] : 0, (int)q3[2],
+                      a[7] == Py_True, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(status);
+}
+
+/* (cache, its device, table or None, its device, q or None, k, v, first, lens, q_out or None) */
+static PyObject* cache4_append(PyObject* self, PyObject* const* a, Py_ssize_t n)
+{
+    long long dev, q3[3], k3[3] = {-1, -1, -1};
+    void *first, *lens, *stream;
+    int type = -1;
+    tllm_b200_heads q, qo, k, v;
+    const tllm_b200_cache4* c;
+    const tllm_b200_rotary_table* t = NULL;
+    if (n != 10 || !f_append || !where(&dev, &stream) || !(c = handle(a[0], a[1], dev, sizeof *c)) ||
+        (a[2] != Py_None && !(t = handle(a[2], a[3], dev, sizeof *t))))
+        Py_RETURN_NONE;
+    k3[1] = c->kv_heads, k3[2] = c->dim;
+    const int queries = a[4] != Py_None;
+    if (!rows3(a[5], dev, &type, k3, &k) || type == TLLM_FP32 || !rows3(a[6], dev, &type, k3, &v) || !sequences(c, a[7], a[8], dev, &first, &lens))
+        Py_RETURN_NONE;
+    q3[0] = k3[0], q3[1] = -1, q3[2] = c->dim;
+    if ((!queries && a[9] != Py_None) || (queries && (!rows3(a[4], dev, &type, q3, &q) || !rows3(a[9] == Py_None ? a[4] : a[9], dev, &type, q3, &qo))))
+        Py_RETURN_NONE;
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = f_append(c, type, t, first, lens, (int)k3[0], queries ? &q : NULL, queries ? &qo : NULL, queries ? (int)q3[1] : 0, &k, &v, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(status);
+}
+
+/* (cache, its device, k or None, v or None, first, lens) */
+static PyObject* cache4_read(PyObject* self, PyObject* const* a, Py_ssize_t n)
+{
+    long long dev, k3[3] = {-1, -1, -1};
+    void *first, *lens, *stream;
+    int type = -1;
+    tllm_b200_heads k, v;
+    const tllm_b200_cache4* c;
+    if (n != 6 || !f_read || !where(&dev, &stream) || !(c = handle(a[0], a[1], dev, sizeof *c)) || (a[2] == Py_None && a[3] == Py_None)) Py_RETURN_NONE;
+    k3[1] = c->kv_heads, k3[2] = c->dim;
+    if ((a[2] != Py_None && !rows3(a[2], dev, &type, k3, &k)) || (a[3] != Py_None && !rows3(a[3], dev, &type, k3, &v)) ||
+        !sequences(c, a[4], a[5], dev, &first, &lens))
+        Py_RETURN_NONE;
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = f_read(c, type, first, lens, (int)k3[0], a[2] != Py_None ? &k : NULL, a[3] != Py_None ? &v : NULL, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(status);
+}
+
+/* (cache, its device, q, out, first, lens, scale, max_new, max_len); the workspace is a tensor of the call's own */
+static PyObject* cache4_attention(PyObject* self, PyObject* const* a, Py_ssize_t n)
+{
+    long long dev, q3[3] = {-1, -1, -1};
+    void *first, *lens, *stream, *ws = NULL;
+    int type = -1;
+    size_t need = 0;
+    tllm_b200_heads q, out;
+    const tllm_b200_cache4* c;
+    if (n != 9 || !f_attention || !where(&dev, &stream) || !(c = handle(a[0], a[1], dev, sizeof *c)) || !PyFloat_CheckExact(a[6])) Py_RETURN_NONE;
+    const int max_new = not_negative(a[7]), max_len = not_negative(a[8]);
+    q3[2] = c->dim;
+    if (max_new < 0 || max_len < 0 || !rows3(a[2], dev, &type, q3, &q) || type == TLLM_FP32 || !rows3(a[3], dev, &type, q3, &out) ||
+        !sequences(c, a[4], a[5], dev, &first, &lens))
+        Py_RETURN_NONE;
+    int status = f_workspace(c, (int)q3[0], (int)q3[1], max_new, max_len, &need);
+    if (status) return PyLong_FromLong(status);
+    PyObject* memory = NULL;
+    if (need) {
+        PyObject* size = PyLong_FromSize_t((need + 1) / 2);               /* q's type has two bytes */
+        memory = size ? PyObject_CallMethodOneArg(a[2], s_new_empty, size) : NULL;
+        Py_XDECREF(size);
+        if (!memory) return NULL;                                         /* out of memory, as torch says it */
+        const long long p = number(method(memory, s_data_ptr));
+        if (p <= 0) {
+            Py_DECREF(memory);
+            Py_RETURN_NONE;
+        }
+        ws = (void*)p;
+    }
+    const float scale = (float)PyFloat_AS_DOUBLE(a[6]);
+    Py_BEGIN_ALLOW_THREADS
+    status = f_attention(c, type, first, lens, (int)q3[0], &q, &out, (int)q3[1], scale, max_new, max_len, ws, need, stream);
+    Py_END_ALLOW_THREADS
+    Py_XDECREF(memory);
+    return PyLong_FromLong(status);
+}
+
+/* (rotary, append, read, attention, workspace addresses, bfloat16, float32, int32), after bind */
+static PyObject* bind_cache4(PyObject* self, PyObject* args)
+{
+    unsigned long long f[5];
+    PyObject *b, *s, *i;
+    if (!PyArg_ParseTuple(args, "KKKKKOOO", &f[0], &f[1], &f[2], &f[3], &f[4], &b, &s, &i)) return NULL;
+    Py_INCREF(b);
+    Py_INCREF(s);
+    Py_INCREF(i);
+    d_types[0] = d_half, d_types[1] = b, d_types[2] = s, d_int32 = i;
+    f_append = (void*)(uintptr_t)f[1];
+    f_read = (void*)(uintptr_t)f[2];
+    f_workspace = (void*)(uintptr_t)f[4];
+    f_attention = (void*)(uintptr_t)f[3];
+    f_rotary = (void*)(uintptr_t)f[0];
+    Py_RETURN_NONE;
+}
+
 /* (gemv, gemv_int8, gemm addresses, current_device, raw_stream, float16, int8, uint8) */
 static PyObject* bind(PyObject* self, PyObject* args)
 {
@@ -151,9 +354,14 @@ static PyMethodDef methods[] = {
     {"gemv_int8_packed", (PyCFunction)(void*)gemv_int8_packed, METH_FASTCALL, NULL},
     {"gemm_packed", (PyCFunction)(void*)gemm_packed, METH_FASTCALL, NULL},
     {"bind", bind, METH_VARARGS, NULL},
+    {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL, NULL},
+    {"cache4_append", (PyCFunction)(void*)cache4_append, METH_FASTCALL, NULL},
+    {"cache4_read", (PyCFunction)(void*)cache4_read, METH_FASTCALL, NULL},
+    {"cache4_attention", (PyCFunction)(void*)cache4_attention, METH_FASTCALL, NULL},
+    {"bind_cache4", bind_cache4, METH_VARARGS, NULL},
     {NULL, NULL, 0, NULL},
 };
-static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostcall", "Operators on prepared weights in one native call.", -1, methods,
+static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostcall", "Operators on prepared weights and on the 4-bit cache in one native call.", -1, methods,
                                     NULL, NULL, NULL, NULL};
 
 PyMODINIT_FUNC PyInit__hostcall(void)
@@ -164,6 +372,10 @@ PyMODINIT_FUNC PyInit__hostcall(void)
     s_get_device = PyUnicode_InternFromString("get_device");
     s_numel = PyUnicode_InternFromString("numel");
     s_data_ptr = PyUnicode_InternFromString("data_ptr");
+    s_shape = PyUnicode_InternFromString("shape");
+    s_stride = PyUnicode_InternFromString("stride");
+    s_new_empty = PyUnicode_InternFromString("new_empty");
+    if (!s_shape || !s_stride || !s_new_empty) return NULL;
     if (!s_is_cuda || !s_dtype || !s_is_contiguous || !s_get_device || !s_numel || !s_data_ptr) return NULL;
     return PyModule_Create(&module);
 }
