@@ -56,19 +56,20 @@ __device__ __forceinline__ Span span_of(const Seqs& s, int b, bool report)
     if (report && (lo < 0 || hi > s.tokens || hi < lo || len < 0 || len > s.rows)) atomicExch(s.err, TLLM_ERR_SHAPE);
     return r;
 }
-// Angle of a pair at a position: the position times the turns a position, as 64-bit fractions of a turn,
-// is exact modulo whole turns; its upper 32 bits are the angle to 2^-32 of a turn.
+// Cosine and sine of a pair at a position, times the amplitude.  The position times the turns a position, as 64-bit fractions of a turn,
+// is exact modulo whole turns; from there on 64 bits until the one rounding (a row's angles are computed once for all of its heads).
 __device__ __forceinline__ void turn(const Rotary& r, unsigned long long turns, int position, float& c, float& s)
 {
-    const unsigned long long phase = turns * (unsigned long long)(long long)position + 0x80000000ull;
-    sincospif((float)(int)(phase >> 32) * 0x1p-31f, &s, &c);
-    c *= r.amplitude;
-    s *= r.inverse ? -r.amplitude : r.amplitude;
+    const long long phase = (long long)(turns * (unsigned long long)(long long)position);
+    double sd, cd;
+    sincospi((double)phase * 0x1p-63, &sd, &cd);
+    c = (float)(cd * (double)r.amplitude);
+    s = (float)(sd * (double)(r.inverse ? -r.amplitude : r.amplitude));
 }
 
-// The turned pair; written out, so that every kernel rounds alike.
-__device__ __forceinline__ float turned_first(float x1, float x2, float2 c) { return fmaf(x1, c.x, -(x2 * c.y)); }
-__device__ __forceinline__ float turned_second(float x1, float x2, float2 c) { return fmaf(x2, c.x, x1 * c.y); }
+// The turned pair: products and sum are FP32 operations of their own, so that every kernel rounds alike and codes follow from the definition.
+__device__ __forceinline__ float turned_first(float x1, float x2, float2 c) { return __fsub_rn(__fmul_rn(x1, c.x), __fmul_rn(x2, c.y)); }
+__device__ __forceinline__ float turned_second(float x1, float x2, float2 c) { return __fadd_rn(__fmul_rn(x2, c.x), __fmul_rn(x1, c.y)); }
 
 template <typename T> __device__ __forceinline__ float as_float(T x);
 template <> __device__ __forceinline__ float as_float<half>(half x) { return __half2float(x); }

@@ -4,9 +4,14 @@
 
 namespace tllm {
 
+// Rows of a key/value head go 16 at once through mma.sync up to 32 of them, and while one tile of 16 a SM takes the call; behind that 256 at once
+// through tcgen05.  Both sides, us, 32 heads over 8: of 64, 6 sequences of 5 tokens behind 3000 21.1 / 27.4, 24 of 8 behind 1000 30.4 / 35.2; of
+// 128, 24 of 8 behind 3000 75 / 83, one of 16 behind 3000 18.6 / 23.6, one of 32 23.4 / 25.0 (64 tiles), 6 of 16 45.7 / 33.8 (192 tiles), 6 of 32
+// behind 200 22.1 / 15.5.
 static bool takes_step(const Cache4& c, int tokens, int heads, int max_new)
 {
-    return (long long)(max_new > 0 && max_new < tokens ? max_new : tokens) * (heads / c.kv_heads) <= 16;
+    const long long rows = (long long)(max_new > 0 && max_new < tokens ? max_new : tokens) * (heads / c.kv_heads);
+    return rows <= 32 || (rows + 15) / 16 * c.batch * c.kv_heads <= 148;
 }
 
 size_t cache4_workspace(const Cache4& c, int tokens, int heads, int max_new, int max_len)

@@ -2,8 +2,7 @@
 //
 // A key/value head's rows (new tokens times the query heads that share it, up to 4, 8 or 16 at once) go through the
 // cache together on mma.sync.  With keys k = l + s c and values alike, scales and lowest values stay outside the products:
-//   scores   sum_groups s (c . q) + l sum q   c . q in integers: codes are bytes after one mask (and a shift for every
-//            other one), a query is 16 bits of its largest entry in the group, as two signed bytes in neighbouring columns
+//   scores   sum_groups s (c . q) + l sum q   c . q in integers: codes, or codes times 16, are bytes after one mask, a query is 16 bits of its largest entry in the group, as two signed bytes in neighbouring columns
 //            of the product (m16n8k32), whose sums are joined exactly.  Positions are the rows of the product.
 //   outputs  sum_p (w s) (c - 8) + sum_p w (l + 8 s)   codes are FP16 numbers after a mask and an addition or
 //            multiplication for two, w s is rounded to FP16 (11 bits of it, with a power of two that follows the largest
@@ -144,18 +143,28 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
         const auto load = [&](int slot) {
             if (issued < j1) {
                 const int left = visible - issued * kStepChunk;            // positions behind hold anything: nothing of them is read
-                const bool full = left >= kStepChunk;
                 const uint32_t at = slot * St::kSlot;
+                if (left >= kStepChunk) {
 #pragma unroll
-                for (int i = 0; i < kPieces; i++) {
-                    const bool valid = full || my_row + i * kSpan < left;
-                    const int off = valid ? i * kSpan * (DIM / 2) : 0;
-                    copy_async<16>(to_codes + at + i * kSpan * (DIM / 2), valid ? k_src + off : a.c.kc, valid);
-                    copy_async<16>(to_codes + at + St::kCodes + i * kSpan * (DIM / 2), valid ? v_src + off : a.c.vc, valid);
+                    for (int i = 0; i < kPieces; i++) {
+                        constexpr int kNext = kSpan * (DIM / 2);
+                        copy_async<16>(to_codes + at + i * kNext, k_src + i * kNext, true);
+                        copy_async<16>(to_codes + at + St::kCodes + i * kNext, v_src + i * kNext, true);
+                    }
+                    copy_async<4 * GR>(to_params + at, kp_src, true);
+                    copy_async<4 * GR>(to_params + at + St::kParams, vp_src, true);
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < kPieces; i++) {
+                        const bool valid = my_row + i * kSpan < left;
+                        const int off = i * kSpan * (DIM / 2);
+                        copy_async<16>(to_codes + at + off, valid ? k_src + off : a.c.kc, valid);
+                        copy_async<16>(to_codes + at + St::kCodes + off, valid ? v_src + off : a.c.vc, valid);
+                    }
+                    const bool valid = lane < left;
+                    copy_async<4 * GR>(to_params + at, valid ? kp_src : a.c.kp, valid);
+                    copy_async<4 * GR>(to_params + at + St::kParams, valid ? vp_src : a.c.vp, valid);
                 }
-                const bool valid = full || lane < left;
-                copy_async<4 * GR>(to_params + at, valid ? kp_src : a.c.kp, valid);
-                copy_async<4 * GR>(to_params + at + St::kParams, valid ? vp_src : a.c.vp, valid);
                 k_src += kStep * (DIM / 2);
                 v_src += kStep * (DIM / 2);
                 kp_src += kStep * GR;
@@ -205,13 +214,13 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                     b[i] = (uint32_t)(g & 1 ? x - hi * 256 : hi) & 0xff;
                 }
                 // bytes as the codes lie in a word: low nibbles 0, 2, 4, 6 are entries 0, 4, 1, 5, high ones 2, 6, 3, 7
-                digits[(k * 2 + w) * 2][lane] = b[0] | b[4] << 8 | b[1] << 16 | b[5] << 24;
-                digits[(k * 2 + w) * 2 + 1][lane] = b[2] | b[6] << 8 | b[3] << 16 | b[7] << 24;
+                digits[k * 4 + w][lane] = b[0] | b[4] << 8 | b[1] << 16 | b[5] << 24;
+                digits[k * 4 + 2 + w][lane] = b[2] | b[6] << 8 | b[3] << 16 | b[7] << 24;
             }
 #pragma unroll
             for (int d = 1; d < 4; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
             // a query that is not finite has no scores
-            if (t == 0 && !(g & 1)) worth[k][g >> 1] = make_float2((float)total, odd ? NAN : top / kDigits * (a.scale * 1.4426950408889634f));
+            if (t == 0 && !(g & 1)) worth[k][g >> 1] = make_float2(16.f * (float)total, odd ? NAN : top / (16.f * kDigits) * (a.scale * 1.4426950408889634f));
         }
         __syncthreads();
         uint32_t qd[NS][GR][2][2];
@@ -290,7 +299,7 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                 }
 #pragma unroll
                 for (int gr = 0; gr < GR; gr++) {
-                    int acc[NS][4] = {};
+                    int low[NS][4] = {}, high[NS][4] = {};                  // of low nibbles, and of high ones sixteen times as large
                     uint2 w[2];
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
@@ -298,17 +307,15 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                         w[u] = *reinterpret_cast<const uint2*>(kc + row * (DIM / 2) + piece * 16 + (t & 1) * 8);
                     }
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const uint32_t w0 = i ? w[0].y : w[0].x, w1 = i ? w[1].y : w[1].x;
-                        const uint32_t a0 = w0 & 0x0f0f0f0fu, a1 = w1 & 0x0f0f0f0fu, a2 = (w0 >> 4) & 0x0f0f0f0fu, a3 = (w1 >> 4) & 0x0f0f0f0fu;
-#pragma unroll
-                        for (int n = 0; n < NS; n++) mma_u8s8(acc[n], a0, a1, a2, a3, qd[n][gr][i][0], qd[n][gr][i][1]);
+                    for (int n = 0; n < NS; n++) {
+                        mma_u8s8(low[n], w[0].x & 0x0f0f0f0fu, w[1].x & 0x0f0f0f0fu, w[0].y & 0x0f0f0f0fu, w[1].y & 0x0f0f0f0fu, qd[n][gr][0][0], qd[n][gr][0][1]);
+                        mma_u8s8(high[n], w[0].x & 0xf0f0f0f0u, w[1].x & 0xf0f0f0f0u, w[0].y & 0xf0f0f0f0u, w[1].y & 0xf0f0f0f0u, qd[n][gr][1][0], qd[n][gr][1][1]);
                     }
 #pragma unroll
                     for (int n = 0; n < NS; n++)
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            const float dot = (float)(acc[n][2 * u] * 256 + acc[n][2 * u + 1]);
+                            const float dot = (float)(low[n][2 * u] * 4096 + low[n][2 * u + 1] * 16 + high[n][2 * u] * 256 + high[n][2 * u + 1]);
                             const float v = fmaf(par[u][gr].x, dot, par[u][gr].y * qsum[n][gr]);
                             s[n][h][u] = gr == 0 ? v * unit_q[n][gr] : fmaf(v, unit_q[n][gr], s[n][h][u]);
                         }
@@ -509,7 +516,10 @@ StepPlan step_plan(const Cache4& c, int tokens, int heads, int max_new, int max_
     p.rows = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
     const long long items = (long long)c.batch * c.kv_heads * ((rows + p.rows - 1) / p.rows);
     const int len = max_len > 0 && max_len < c.rows ? max_len : c.rows;
-    p.whole = len <= 512;
+    // A tile's positions stay in one CTA while that takes no longer than a second launch and what it waits for.  Both ways, us, one / 48
+    // sequences of 32 heads over 8: heads of 128 behind 300 6.4 / 14.2 in one CTA, 12.1 / 17.2 cut; behind 800 8.8 / 20.1, 12.7 / 24.3; behind
+    // 1200 10.3 / 24.0, 12.4 / 27.6; behind 2000 13.7 / 34.0, 11.4 / 37.5; heads of 64 behind 2000 9.3 / 21.5, 9.5 / 25.3.
+    p.whole = len <= 160000 / c.dim;
     p.ctas = p.whole ? (int)(items < 65536 ? items : 65536) : p.rows == 16 ? 148 : 296;
     p.bytes = p.whole ? 0 : join_bytes(c.dim, p.rows, p.ctas);
     return p;
