@@ -391,12 +391,13 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
                 const int at = (warp & 3) * 32 + k * kAtOnce + lane / kLanes;
                 return qs + i * P::kOperand + (lane % kLanes >> 3) * kBlock + at * 128 + (((lane & 7) ^ (at & 7)) << 4);
             };
+            int at0 = (warp & 3) * 32 + lane / kLanes, tok = (w.tile * kRows + i * kTile + at0) / w.per, sub = (w.tile * kRows + i * kTile + at0) - tok * w.per;
 #pragma unroll 2
-            for (int k = 0; k < 32 / kAtOnce; k++) {
-                const int at = (warp & 3) * 32 + k * kAtOnce + lane / kLanes;
-                const unsigned from = w.tile * kRows + i * kTile + (at < tile_rows ? at : 0), tok = from / (unsigned)w.per;
-                const T* src = q.p + (size_t)(w.span.row0 + tok) * q.ld + (size_t)(w.head * w.per + from - tok * w.per) * DIM + lane % kLanes * 8;
-                copy_async<16>(smem_u32(piece(k)), src, at < tile_rows);
+            for (int k = 0; k < 32 / kAtOnce; k++, at0 += kAtOnce, sub += kAtOnce) {
+                for (; sub >= w.per; sub -= w.per) tok++;
+                const bool valid = at0 < tile_rows;
+                const T* src = q.p + (size_t)(w.span.row0 + (valid ? tok : 0)) * q.ld + (size_t)(w.head * w.per + (valid ? sub : 0)) * DIM + lane % kLanes * 8;
+                copy_async<16>(smem_u32(piece(k)), src, valid);
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             if (!std::is_same<T, half>::value || sign) {

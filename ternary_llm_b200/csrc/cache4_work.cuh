@@ -58,8 +58,8 @@ int launch_cache4_join(const Cache4Call& a, Rows<T> out, int rows, int ctas, cud
 // Units are counted in 32 bits (work_fits).
 template <int R, int CHUNK>
 struct Work {
-    static constexpr int kFixed = CHUNK == kStepChunk ? 8 : 2;
-    static constexpr int kLeast = CHUNK == kStepChunk ? 24 : 4;            // units that a CTA takes at least where work is cut
+    static constexpr int kFixed = CHUNK == kStepChunk ? 20 : 2;
+    static constexpr int kLeast = CHUNK == kStepChunk ? 36 : 4;            // units that a CTA takes at least where work is cut
     struct Start {
         int x, to, share, b, head, tile, offset;
     };
@@ -212,7 +212,7 @@ struct Work {
 // Whether the units of a call fit 31 bits, whatever first and lens hold (even all rows in every sequence).
 inline bool work_fits(const Cache4& c, int tokens, int heads, int rows, int chunk)
 {
-    const double tiles = (double)tokens * (heads / c.kv_heads) / rows + 1, units = (double)c.rows / chunk + 10;
+    const double tiles = (double)tokens * (heads / c.kv_heads) / rows + 1, units = (double)c.rows / chunk + 22;
     return tiles * units * c.batch * c.kv_heads < 2e9;
 }
 
