@@ -25,9 +25,8 @@ TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 SCALINGS = {"linear": 1, "ntk": 2, "yarn": 3, "llama3": 4}
 
 
-def rotary_frequencies(rot_dim: int, base: float, scaling: dict | None = None):
-    """(angles a position of the rot_dim / 2 pairs, factor of the result).  scaling: type "linear" or "ntk"
-    (factor), "yarn" (factor, original length, beta_fast, beta_slow) or "llama3" (factor, original, low, high)."""
+def _frequencies(rot_dim: int, base: float, scaling: dict | None):
+    """(C array, factor of the result)."""
     s = dict(scaling or {})
     kind = s.pop("type", None)
     if scaling is not None and kind not in SCALINGS:
@@ -43,19 +42,26 @@ def rotary_frequencies(rot_dim: int, base: float, scaling: dict | None = None):
         raise ValueError(f"scaling: unknown {', '.join(map(repr, s))}")
     f, amplitude = (ctypes.c_double * max(1, rot_dim // 2))(), ctypes.c_float()
     _lib.check(_lib.lib().tllm_b200_rotary_frequencies(rot_dim, base, ctypes.byref(d), f, ctypes.byref(amplitude)))
-    return list(f), amplitude.value
+    return f, amplitude.value
+
+
+def _turns(frequencies, n: int):
+    out = (ctypes.c_uint64 * max(1, n))()
+    _lib.check(_lib.lib().tllm_b200_rotary_turns(frequencies, n, out))
+    return out
+
+
+def rotary_frequencies(rot_dim: int, base: float, scaling: dict | None = None):
+    """(angles a position of the rot_dim / 2 pairs, factor of the result).  scaling: type "linear" or "ntk"
+    (factor), "yarn" (factor, original length, beta_fast, beta_slow) or "llama3" (factor, original, low, high)."""
+    f, amplitude = _frequencies(rot_dim, base, scaling)
+    return list(f), amplitude
 
 
 def rotary_turns(frequencies):
     """The frequencies in turns a position, as 64-bit fractions."""
     n = len(frequencies)
-    return list(_turns(frequencies, n))[:n]
-
-
-def _turns(frequencies, n: int):
-    out = (ctypes.c_uint64 * max(1, n))()
-    _lib.check(_lib.lib().tllm_b200_rotary_turns((ctypes.c_double * max(1, n))(*frequencies), n, out))
-    return out
+    return list(_turns((ctypes.c_double * max(1, n))(*frequencies), n))[:n]
 
 
 class RotaryTable:
@@ -65,17 +71,21 @@ class RotaryTable:
     def __init__(self, rot_dim: int, base: float = 10000.0, half: bool = True, scaling: dict | None = None, frequencies=None,
                  amplitude: float | None = None, device=None):
         if frequencies is None:
-            frequencies, own = rotary_frequencies(rot_dim, base, scaling)
+            f, own = _frequencies(rot_dim, base, scaling)
         else:
-            frequencies, own = [float(f) for f in frequencies], 1.0
+            f, own = (ctypes.c_double * max(1, len(frequencies)))(*frequencies), 1.0
             if 2 * len(frequencies) != rot_dim:
                 raise ValueError(f"{len(frequencies)} frequencies for {rot_dim} entries")
-        self.rot_dim, self.half, self.frequencies = rot_dim, half, frequencies
+        self.rot_dim, self.half, self._f = rot_dim, half, f
         self.amplitude = own if amplitude is None else float(amplitude)
-        turns = _turns(frequencies, rot_dim // 2)
-        self.turns = torch.frombuffer(turns, dtype=torch.int64, count=rot_dim // 2).to("cuda" if device is None else device, copy=True)
+        turns = torch.frombuffer(_turns(f, rot_dim // 2), dtype=torch.int64, count=rot_dim // 2)
+        self.turns = turns.clone() if device is not None and torch.device(device).type == "cpu" else turns.to("cuda" if device is None else device)
         self._device = self.turns.get_device()
         self._bytes = bytes(_lib.RotaryTableDesc(self.turns.data_ptr(), rot_dim, int(half), self.amplitude))
+
+    @property
+    def frequencies(self):
+        return list(self._f)[:self.rot_dim // 2]
 
     def _desc(self):
         return _lib.RotaryTableDesc(_chk(self.turns, torch.int64, "turns", self.rot_dim // 2), self.rot_dim, int(self.half), self.amplitude)

@@ -580,10 +580,15 @@ PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int 
     PromptPlan p;
     const int per = heads / c.kv_heads, most = max_new > 0 && max_new < tokens ? max_new : tokens;
     const long long tiles = ((long long)most * per + kRows - 1) / kRows, pairs = (long long)c.batch * c.kv_heads;
-    // tiles of rows that there are at most, and at most in all
-    const long long all = ((long long)tokens * per + kRows - 1) / kRows * c.kv_heads + pairs;
     const long long grid = tiles * pairs < (1 << 20) ? tiles * pairs : (1 << 20) / pairs * pairs;
-    p.whole = all >= 222;
+    // A tile of rows stays in one CTA unless the longest would keep its SM busy for more than seven tiles of positions (some 2 us each) after
+    // the others are done, which is what cutting costs in records and a second launch.  Both ways, us, 32 heads over 8: of 128, a prompt of 1500
+    // 39 whole, 57 cut, 2000 52 / 74; of 64, four prompts of 700 38 / 51; 512 tokens behind 16000 are 64 tiles of rows of 129 tiles each,
+    // which whole would take twice the 158 us.
+    const int len = max_len > 0 && max_len < c.rows ? max_len : c.rows;
+    const double longest = (len + kTile - 1) / kTile, mean = longest - (most < len ? most : len) / (2.0 * kTile);
+    const double rows = (double)tokens * per / kRows > (double)c.batch ? (double)tokens * per / kRows : (double)c.batch;
+    p.whole = longest - rows * c.kv_heads * mean / 148 <= 7;
     p.ctas = p.whole ? (int)(grid < pairs ? pairs : grid) : 148;
     p.bytes = p.whole ? 0 : join_bytes(c.dim, kRows, p.ctas);
     return p;

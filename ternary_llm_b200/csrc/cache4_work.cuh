@@ -58,8 +58,8 @@ int launch_cache4_join(const Cache4Call& a, Rows<T> out, int rows, int ctas, cud
 // Units are counted in 32 bits (work_fits).
 template <int R, int CHUNK>
 struct Work {
-    static constexpr int kFixed = CHUNK == kStepChunk ? 20 : 2;
-    static constexpr int kLeast = CHUNK == kStepChunk ? 36 : 4;            // units that a CTA takes at least where work is cut
+    static constexpr int kFixed = CHUNK == kStepChunk ? 20 : 4;
+    static constexpr int kLeast = CHUNK == kStepChunk ? 36 : 6;            // units that a CTA takes at least where work is cut
     struct Start {
         int x, to, share, b, head, tile, offset;
     };

@@ -318,6 +318,37 @@ def test_prompts(dtype, before, new, heads, kv_heads, dim):
     attention_case(dtype, before, new, heads, kv_heads, dim)
 
 
+@pytest.mark.parametrize("before,new,heads,kv_heads,dim", [
+    ([1249], [1], 8, 2, 128), ([1250], [1], 8, 2, 128), ([2499], [1], 4, 1, 64), ([2500], [1], 4, 1, 64),                  # one CTA a head, or several
+    ([2600, 40], [1, 1], 8, 1, 128), ([2600, 40], [1, 1], 16, 1, 64), ([2600, 40], [2, 1], 4, 1, 64),                      # tiles of 4, 8 and 16 rows, cut
+    ([1300], [8], 8, 2, 128), ([1300], [9], 8, 2, 128), ([0] * 25, [33] * 25, 6, 6, 64), ([0] * 24, [33] * 24, 6, 6, 64),  # few rows and many
+    ([900], [140], 4, 1, 64), ([1800], [140], 4, 1, 64), ([1800], [300], 5, 1, 128), ([4000, 5], [129, 200], 2, 2, 64)])   # prompts whole and cut
+def test_both_sides_of_the_lines_between_ways(before, new, heads, kv_heads, dim):
+    for dtype in TYPES:
+        attention_case(dtype, before, new, heads, kv_heads, dim)
+
+
+@pytest.mark.parametrize("new", [1, 7, 150])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30])
+def test_scales_that_are_not_positive(new, scale):
+    attention_case(torch.float16, [90], [new], 8, 2, 64, scale=scale)
+    attention_case(torch.bfloat16, [2000], [new], 4, 1, 128, scale=scale)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_the_native_call_and_the_other_way_agree(new):
+    """A scale that is no plain float takes the checks in Python and ctypes."""
+    c, q, out = attention_case(torch.float16, [3000], [new], 8, 2, 128, scale=1.0)
+    other = torch.full_like(q[:new], 7.0)
+    ops.attention(c, q[:new], other, ints(0, new), ints(3000 + new), scale=1, max_new=new, max_len=3000 + new)
+    assert torch.equal(other, out[:new])
+    table, x = ops.RotaryTable(128), q[:new].contiguous()
+    position, y, z = torch.arange(new, dtype=torch.int32, device="cuda"), torch.empty_like(x), torch.empty_like(x)
+    ops.rotary(x, None, position, table, y)
+    ops.rotary(x, None, position, table, z, inverse=0)
+    assert torch.equal(y, z)
+
+
 @pytest.mark.parametrize("new", [[1, 1], [3, 40], [200, 130]])
 @pytest.mark.parametrize("new_hint,len_hint", [(0, 0), (1, 2700), (5, 0), (1000, 100000), (90, 2700), (1, 0)])
 def test_hints_do_not_matter(new, new_hint, len_hint):
@@ -404,7 +435,7 @@ def test_same_result_every_time_and_on_two_streams():
     """Bit for bit: two runs, two streams at once, a captured graph replayed while another runs."""
     gen = torch.Generator(device="cuda").manual_seed(3)
     calls = []
-    for before, new in (([9000, 100], [1, 1]), ([300], [700]), ([4000, 3], [4, 2])):
+    for before, new in (([9000, 100], [1, 1]), ([300], [700]), ([4000, 3], [4, 2]), ([6000], [200])):
         lens = [a + n for a, n in zip(before, new)]
         c = random_cache(gen, len(new), 2, max(lens), 128, lens)
         first, lens_dev, tokens = layout(before, new)
