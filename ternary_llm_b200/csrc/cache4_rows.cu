@@ -5,7 +5,9 @@
 // 0..15; the limit keeps s c + l inside FP16.  Both differences and quotients are single FP32 operations, so the codes
 // follow from the rounded activations alone.  Eight lanes have a group, a lane eight neighbouring values: 16 bytes in,
 // a word of codes out.  The keys and values of a head of a row stay with the same lanes, which mark a NaN in either.
-// Bound by the bytes for many rows, by the chain of loads (sequence, position, angles, row) for a few.
+// Bound by the chain of a CTA (sequence and position, angles, row): three FP16 prompts of 3982 rows in all, 32 heads of 64
+// over 8, 46 MB, take 19 us with four rows a CTA and four CTAs an SM, 24.5 with two CTAs, 22 with eight rows, 48 with one
+// row; 24 rows of 128 take 4.8.
 #include "cache4.cuh"
 #include "launch.cuh"
 
@@ -70,35 +72,39 @@ __device__ __forceinline__ float max8(float v)
     return v;
 }
 
-// The codes and (s, l) of the group that eight lanes hold.
+// The codes and (s, l) of the group that eight lanes hold.  The quotient is the correctly rounded one in three operations:
+// a product with the reciprocal and one correction by the exact remainder (Markstein 1990) is within 2^-45 of the true one,
+// relative to it, and a quotient by the 11 bits of s lies no nearer than 2^-36 to the middle of two FP32 values.  Four
+// codes are put together as one FP32 number.
 __device__ __forceinline__ void write_group(uint8_t* codes, half2* params, size_t row, int words, int lane_of_row, const float (&x)[8], bool bad, bool write)
 {
     float v[8], low = INFINITY, high = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        v[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -TLLM_CACHE4_LIMIT), TLLM_CACHE4_LIMIT);
+        v[i] = fminf(fmaxf(x[i], -TLLM_CACHE4_LIMIT), TLLM_CACHE4_LIMIT);
         low = fminf(low, v[i]);
         high = fmaxf(high, v[i]);
     }
     const half l = __float2half_rn(-max8(-low));
     const float lf = __half2float(l);
     const half s = __float2half_rn((max8(high) - lf) / 15.f);
-    const float sf = __half2float(s);
-    uint32_t word = 0;
+    const float sf = __half2float(s), r = sf > 0.f ? __frcp_rn(sf) : 0.f;
+    float c[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const float c = sf > 0.f ? fminf(fmaxf(rintf((v[i] - lf) / sf), 0.f), 15.f) : 0.f;
-        word |= (uint32_t)c << (4 * (i >> 1) + 16 * (i & 1));
+        const float t = v[i] - lf, q = t * r;
+        c[i] = fminf(fmaxf(rintf(fmaf(fmaf(-q, sf, t), r, q)), 0.f), 15.f);
     }
     if (!write) return;
-    reinterpret_cast<uint32_t*>(codes)[row * words + lane_of_row] = word;
+    const float even = fmaf(4096.f, c[6], fmaf(256.f, c[4], fmaf(16.f, c[2], c[0]))), odd = fmaf(4096.f, c[7], fmaf(256.f, c[5], fmaf(16.f, c[3], c[1])));
+    reinterpret_cast<uint32_t*>(codes)[row * words + lane_of_row] = (uint32_t)even | (uint32_t)odd << 16;
     if ((lane_of_row & 7) == 0)
         params[row * (words / 8) + lane_of_row / 8] = bad ? __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff)) : __halves2half2(s, l);
 }
 
 // blockIdx.y = 0: keys and values, 1: queries.
 template <typename T, int DIM, int ROWS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 cache4_append_kernel(const AppendArgs<T> a)
 {
     __shared__ Places<ROWS> at;
@@ -129,13 +135,14 @@ cache4_append_kernel(const AppendArgs<T> a)
     pdl_wait();
     // the rows are on their way while their places and angles are found
     const bool queries = blockIdx.y == 1;
+    const unsigned long long first_turn = tid < ROWS * pairs ? a.r.turns[tid % pairs] : 0;
     if (!queries) load_kv(tid / kLanes);
     else if (whole && h < a.heads) load();
     find_places<ROWS>(a.s, row0, at);
     __syncthreads();
     for (int i = tid; i < ROWS * pairs; i += kThreads) {
         const int r = i / pairs, p = i % pairs;
-        turn(a.r, a.r.turns[p], at.position[r], cs[r][p].x, cs[r][p].y);
+        turn(a.r, i == tid ? first_turn : a.r.turns[p], at.position[r], cs[r][p].x, cs[r][p].y);
     }
     __syncthreads();
     if (queries) {
@@ -221,6 +228,13 @@ cache4_append_kernel(const AppendArgs<T> a)
             bad = bad || k.v[e] != k.v[e] || v.v[e] != v.v[e];
         }
         bad = __ballot_sync(0xffffffffu, bad) >> ((tid & 31) / kLanes * kLanes) & (kLanes == 32 ? 0xffffffffu : (1u << kLanes) - 1);
+        if (bad) {                                         // a NaN counts as 0
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if (k.v[e] != k.v[e]) k.v[e] = 0.f;
+                if (v.v[e] != v.v[e]) v.v[e] = 0.f;
+            }
+        }
         const size_t to = write ? cache_row(a.c, at.seq[r], g, at.position[r]) : 0;
         write_group(a.c.kc, a.c.kp, to, DIM / 8, lane, k.v, bad, write);
         write_group(a.c.vc, a.c.vp, to, DIM / 8, lane, v.v, false, write);
