@@ -17,7 +17,8 @@
  * first[0] and from first[batch] on are left alone.  A row whose position would be negative is padding:
  * nothing is written for it, and its attention is 0.  first that does not rise or leaves 0..tokens, or
  * lens outside 0..rows, is cut to those limits and raises TLLM_ERR_SHAPE at the next
- * tllm_b200_check_device_errors; nothing outside the tensors is read or written.
+ * tllm_b200_check_device_errors; nothing outside the tensors is read or written.  (Where first falls,
+ * attention may leave rows out.)
  *
  * Activations: consecutive heads of a row lie behind one another, rows are ld elements apart, on 16-byte
  * boundaries.  All calls may be captured into graphs (once the library has been used on the device) and keep
@@ -75,7 +76,7 @@ typedef struct tllm_b200_heads {
 
 /* (x1, x2) -> a (x1 cos - x2 sin, x2 cos + x1 sin) with the angles of positions[row]; `inverse` turns the
  * other way (the gradient of this operator).  k and k_out may be NULL (kv_heads 0).  An output may be its
- * input, else they must not overlap.  dim: a multiple of 8 (FP32: of 4) up to 512. */
+ * own input, else outputs must not overlap anything.  dim: a multiple of 8 (FP32: of 4) up to 512. */
 int tllm_b200_rotary(int type, const tllm_b200_rotary_table* table, const int* positions, int tokens, const tllm_b200_heads* q,
                      const tllm_b200_heads* q_out, int heads, const tllm_b200_heads* k, const tllm_b200_heads* k_out, int kv_heads, int dim,
                      int inverse, void* stream);

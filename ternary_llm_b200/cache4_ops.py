@@ -64,7 +64,17 @@ def rotary_turns(frequencies):
     return list(_turns((ctypes.c_double * max(1, n))(*frequencies), n))[:n]
 
 
-class RotaryTable:
+class _Fixed:
+    """What native calls keep the addresses of: set once."""
+    _bytes = None
+
+    def __setattr__(self, name, value):
+        if self._bytes is not None:
+            raise AttributeError(f"{type(self).__name__}.{name} cannot be changed: make another {type(self).__name__}")
+        object.__setattr__(self, name, value)
+
+
+class RotaryTable(_Fixed):
     """Rotary positions of the first rot_dim entries of a head.  half: pairs (i, i + rot_dim / 2), else (2 i, 2 i + 1).
     frequencies: angles a position, instead of base and scaling; amplitude: factor of the result (default: the scaling's)."""
 
@@ -83,6 +93,9 @@ class RotaryTable:
         self._device = self.turns.get_device()
         self._bytes = bytes(_lib.RotaryTableDesc(self.turns.data_ptr(), rot_dim, int(half), self.amplitude))
 
+    def __reduce__(self):
+        return RotaryTable, (self.rot_dim, 0.0, self.half, None, self.frequencies, self.amplitude, str(self.turns.device))
+
     @property
     def frequencies(self):
         return list(self._f)[:self.rot_dim // 2]
@@ -91,7 +104,7 @@ class RotaryTable:
         return _lib.RotaryTableDesc(_chk(self.turns, torch.int64, "turns", self.rot_dim // 2), self.rot_dim, int(self.half), self.amplitude)
 
 
-class Cache4:
+class Cache4(_Fixed):
     """Codes uint8 [batch, kv_heads, rows, dim / 2] and params float16 [batch, kv_heads, rows, dim / 64, 2] of keys and values."""
 
     def __init__(self, k_codes, k_params, v_codes, v_params):
@@ -112,6 +125,9 @@ class Cache4:
             k_codes.dtype == v_codes.dtype == torch.uint8 and k_params.dtype == v_params.dtype == torch.float16
         self._device = k_codes.get_device() if fit else -1
         self._bytes = bytes(_lib.Cache4Desc(*(t.data_ptr() for t in all4), self.batch, self.kv_heads, self.rows, self.dim)) if fit else b""
+
+    def __reduce__(self):
+        return Cache4, (self.k_codes, self.k_params, self.v_codes, self.v_params)
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, rows: int, dim: int, device=None):

@@ -2,12 +2,15 @@
 // and dispatch to rotary.cu, cache4_rows.cu and cache4_attention.cu.
 #include <climits>
 #include <cmath>
+#include <utility>
 
 #include "cache4.cuh"
 
 using namespace tllm;
 
 namespace {
+
+constexpr int kMostHeads = 4096, kMostTokens = INT_MAX - 16;
 
 inline bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 inline size_t type_size(int type) { return type == TLLM_FP32 ? 4 : 2; }
@@ -27,18 +30,18 @@ int check_rows(const char* fn, const char* name, const tllm_b200_heads* x, int t
     return TLLM_OK;
 }
 
-// An output is its input, or lies apart from it.
-int check_apart(const char* fn, const char* name, const tllm_b200_heads* x, const tllm_b200_heads* y, int type, int tokens, int heads, int dim)
+// Rows of an output, and those of an input or another output: the same where that is allowed, or apart.
+int check_apart(const char* fn, const char* name, const tllm_b200_heads* x, int x_heads, const tllm_b200_heads* y, int y_heads, int type, int tokens, int dim,
+                bool same)
 {
-    if (tokens == 0 || (x->p == y->p && (x->ld == y->ld || tokens == 1))) return TLLM_OK;
-    const uintptr_t a = reinterpret_cast<uintptr_t>(x->p), b = reinterpret_cast<uintptr_t>(y->p);
-    const size_t width = (size_t)heads * dim * type_size(type);
-    const size_t na = (size_t)(tokens - 1) * x->ld * type_size(type) + width, nb = (size_t)(tokens - 1) * y->ld * type_size(type) + width;
-    if (a + na <= b || b + nb <= a) return TLLM_OK;
+    if (tokens == 0 || (same && x->p == y->p && (x->ld == y->ld || tokens == 1))) return TLLM_OK;
+    if (x->p > y->p) std::swap(x, y), std::swap(x_heads, y_heads);
+    const size_t one = type_size(type), off = reinterpret_cast<uintptr_t>(y->p) - reinterpret_cast<uintptr_t>(x->p), step = (size_t)x->ld * one;
+    const size_t width = (size_t)x_heads * dim * one, other = (size_t)y_heads * dim * one;
+    if (off >= (size_t)(tokens - 1) * step + width) return TLLM_OK;
     // rows between rows of the other, equally far apart
-    const size_t step = (size_t)x->ld * type_size(type), off = (a > b ? a - b : b - a) % step;
-    if (x->ld == y->ld && off >= width && off + width <= step) return TLLM_OK;
-    return fail(TLLM_ERR_SHAPE, "%s: %s overlaps its output", fn, name);
+    if (tokens > 1 && x->ld == y->ld && off % step >= width && off % step + other <= step) return TLLM_OK;
+    return fail(TLLM_ERR_SHAPE, "%s: %s overlaps an output", fn, name);
 }
 
 int check_table(const char* fn, const tllm_b200_rotary_table* t, int dim, int inverse, Rotary* r)
@@ -67,7 +70,7 @@ int check_cache(const char* fn, const tllm_b200_cache4* c, Cache4* v)
 int check_seqs(const char* fn, const int* first, const int* lens, int tokens, const Cache4& c, Seqs* s)
 {
     if (c.batch > 0 && (!first || !lens)) return fail(TLLM_ERR_NULL, "%s: first or lens is null", fn);
-    if (tokens < 0) return fail(TLLM_ERR_SHAPE, "%s: tokens=%d", fn, tokens);
+    if (tokens < 0 || tokens > kMostTokens) return fail(TLLM_ERR_SHAPE, "%s: tokens=%d", fn, tokens);
     if (misaligned(first, 4) || misaligned(lens, 4)) return fail(TLLM_ERR_ALIGN, "%s: first and lens must be 4-byte aligned", fn);
     *s = Seqs{first, lens, c.batch, tokens, c.rows, nullptr};
     return TLLM_OK;
@@ -84,8 +87,6 @@ template <typename T> Rows<T> out(const tllm_b200_heads* x) { return x ? Rows<T>
 
 inline cudaStream_t S(void* s) { return static_cast<cudaStream_t>(s); }
 
-constexpr int kMostHeads = 4096;
-
 }  // namespace
 
 extern "C" {
@@ -98,15 +99,18 @@ int tllm_b200_rotary(int type, const tllm_b200_rotary_table* table, const int* p
     if (!table || (!positions && tokens > 0)) return fail(TLLM_ERR_NULL, "rotary: null pointer");
     int st = check_type(fn, type, true);
     if (st) return st;
-    if (tokens < 0 || heads < 1 || kv_heads < 0 || heads > kMostHeads || kv_heads > kMostHeads || dim < 8 || dim > 512 || dim * type_size(type) % 16)
+    if (tokens < 0 || tokens > kMostTokens || heads < 1 || kv_heads < 0 || heads > kMostHeads || kv_heads > kMostHeads || dim < 8 || dim > 512 || dim * type_size(type) % 16)
         return fail(TLLM_ERR_SHAPE, "rotary: tokens=%d heads=%d/%d dim=%d", tokens, heads, kv_heads, dim);
     if ((k != nullptr) != (kv_heads > 0) || (k != nullptr) != (k_out != nullptr)) return fail(TLLM_ERR_NULL, "rotary: k, k_out and kv_heads go together");
     Rotary r;
     if ((st = check_table(fn, table, dim, inverse != 0, &r)) || (st = check_rows(fn, "q", q, type, tokens, heads, dim)) ||
-        (st = check_rows(fn, "q_out", q_out, type, tokens, heads, dim)) || (st = check_apart(fn, "q", q, q_out, type, tokens, heads, dim)))
+        (st = check_rows(fn, "q_out", q_out, type, tokens, heads, dim)) || (st = check_apart(fn, "q", q, heads, q_out, heads, type, tokens, dim, true)))
         return st;
     if (k && ((st = check_rows(fn, "k", k, type, tokens, kv_heads, dim)) || (st = check_rows(fn, "k_out", k_out, type, tokens, kv_heads, dim)) ||
-              (st = check_apart(fn, "k", k, k_out, type, tokens, kv_heads, dim))))
+              (st = check_apart(fn, "k", k, kv_heads, k_out, kv_heads, type, tokens, dim, true)) ||
+              (st = check_apart(fn, "k", k, kv_heads, q_out, heads, type, tokens, dim, false)) ||
+              (st = check_apart(fn, "q", q, heads, k_out, kv_heads, type, tokens, dim, false)) ||
+              (st = check_apart(fn, "k_out", k_out, kv_heads, q_out, heads, type, tokens, dim, false))))
         return st;
     if (misaligned(positions, 4)) return fail(TLLM_ERR_ALIGN, "rotary: positions must be 4-byte aligned");
     if ((st = check_device())) return st;
@@ -133,7 +137,9 @@ int tllm_b200_cache4_append(const tllm_b200_cache4* cache, int type, const tllm_
     if (heads < 0 || heads > kMostHeads || c.kv_heads > kMostHeads) return fail(TLLM_ERR_SHAPE, "cache4_append: heads=%d/%d", heads, c.kv_heads);
     if ((q != nullptr) != (heads > 0) || (q != nullptr) != (q_out != nullptr)) return fail(TLLM_ERR_NULL, "cache4_append: q, q_out and heads go together");
     if (q && ((st = check_rows(fn, "q", q, type, tokens, heads, c.dim)) || (st = check_rows(fn, "q_out", q_out, type, tokens, heads, c.dim)) ||
-              (st = check_apart(fn, "q", q, q_out, type, tokens, heads, c.dim))))
+              (st = check_apart(fn, "q", q, heads, q_out, heads, type, c.batch ? tokens : 0, c.dim, true)) ||
+              (st = check_apart(fn, "k", k, c.kv_heads, q_out, heads, type, c.batch ? tokens : 0, c.dim, false)) ||
+              (st = check_apart(fn, "v", v, c.kv_heads, q_out, heads, type, c.batch ? tokens : 0, c.dim, false))))
         return st;
     if ((st = check_device()) || (st = error_flag(&s))) return st;
     if (type == TLLM_FP16) return launch_cache4_append<half>(c, r, s, in<half>(q), out<half>(q_out), heads, in<half>(k), in<half>(v), S(stream));
@@ -150,7 +156,8 @@ int tllm_b200_cache4_read(const tllm_b200_cache4* cache, int type, const int* fi
     if ((st = check_type(fn, type, true)) || (st = check_cache(fn, cache, &c)) || (st = check_seqs(fn, first, lens, tokens, c, &s))) return st;
     if (!k && !v) return fail(TLLM_ERR_NULL, "cache4_read: neither k nor v");
     if (c.kv_heads > kMostHeads) return fail(TLLM_ERR_SHAPE, "cache4_read: heads=%d", c.kv_heads);
-    if ((k && (st = check_rows(fn, "k", k, type, tokens, c.kv_heads, c.dim))) || (v && (st = check_rows(fn, "v", v, type, tokens, c.kv_heads, c.dim))))
+    if ((k && (st = check_rows(fn, "k", k, type, tokens, c.kv_heads, c.dim))) || (v && (st = check_rows(fn, "v", v, type, tokens, c.kv_heads, c.dim))) ||
+        (k && v && (st = check_apart(fn, "k", k, c.kv_heads, v, c.kv_heads, type, c.batch ? tokens : 0, c.dim, false))))
         return st;
     if ((st = check_device()) || (st = error_flag(&s))) return st;
     if (type == TLLM_FP16) return launch_cache4_read<half>(c, s, out<half>(k), out<half>(v), S(stream));
@@ -187,9 +194,8 @@ int tllm_b200_cache4_attention(const tllm_b200_cache4* cache, int type, const in
     int st;
     if ((st = check_type(fn, type, false)) || (st = check_cache(fn, cache, &a.c)) || (st = check_seqs(fn, first, lens, tokens, a.c, &a.s)) ||
         (st = check_heads(fn, a.c, tokens, heads, max_new, max_len)) || (st = check_rows(fn, "q", q, type, tokens, heads, a.c.dim)) ||
-        (st = check_rows(fn, "out", out_rows, type, tokens, heads, a.c.dim)) || (st = check_apart(fn, "q", q, out_rows, type, tokens, heads, a.c.dim)))
+        (st = check_rows(fn, "out", out_rows, type, tokens, heads, a.c.dim)) || (st = check_apart(fn, "q", q, heads, out_rows, heads, type, a.c.batch ? tokens : 0, a.c.dim, false)))
         return st;
-    if (tokens > 0 && a.c.batch > 0 && q->p == out_rows->p) return fail(TLLM_ERR_SHAPE, "cache4_attention: q overlaps its output");
     if (!std::isfinite(scale)) return fail(TLLM_ERR_SHAPE, "cache4_attention: scale %g", scale);
     a.heads = heads;
     a.scale = scale;

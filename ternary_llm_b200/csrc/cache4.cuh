@@ -44,6 +44,7 @@ struct Seqs {
 // Sequence b of a call: n activation rows from row0 on at positions len - n .. len - 1.
 struct Span {
     int row0, n, len;
+    bool falls;                        // first does: sequences may share rows
     __device__ __forceinline__ int position(int i) const { return len - n + i; }
 };
 __device__ __forceinline__ Span span_of(const Seqs& s, int b, bool report)
@@ -53,6 +54,7 @@ __device__ __forceinline__ Span span_of(const Seqs& s, int b, bool report)
     r.row0 = min(max(lo, 0), s.tokens);
     r.n = max(min(max(hi, 0), s.tokens) - r.row0, 0);
     r.len = min(max(len, 0), s.rows);
+    r.falls = hi < lo;
     if (report && (lo < 0 || hi > s.tokens || hi < lo || len < 0 || len > s.rows)) atomicExch(s.err, TLLM_ERR_SHAPE);
     return r;
 }

@@ -25,7 +25,7 @@ int launch_cache4_attention(const Cache4Call& a, Rows<const T> q, Rows<T> out, c
 {
     if (a.s.tokens == 0 || a.s.batch == 0) return TLLM_OK;
     const bool step = takes_step(a.c, a.s.tokens, a.heads, a.max_new);
-    if (!work_fits(a.c, a.s.tokens, a.heads, step ? 4 : kPromptRows, step ? kStepChunk : kPromptChunk))
+    if (!work_fits(a, step ? 4 : kPromptRows, step ? kStepChunk : kPromptChunk))
         return fail(TLLM_ERR_SIZE, "cache4_attention: %d rows of %d heads over %d positions", a.s.tokens, a.heads, a.c.rows);
     if (step)
         return launch_cache4_step<T>(a, q, out, step_plan(a.c, a.s.tokens, a.heads, a.max_new, a.max_len), stream);

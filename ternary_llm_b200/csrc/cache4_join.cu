@@ -1,8 +1,10 @@
 // Attention over the 4-bit key/value cache: tiles of rows whose positions several CTAs took, joined from the CTAs'
 // records (maxima, sums of weights, outputs that are not divided by them).
 //
-// A CTA here for each that has the first chunk of a shared tile: weights of all records first, then their outputs, every load independent of the others.  A thread has four channels of
-// a row and every kParts-th record; the parts meet in shared memory.  The order of all sums is fixed.
+// A CTA here for each that has the first chunk of a shared tile: weights of all records first, then their outputs, every
+// load independent of the others.  A thread has four channels of a row and every kParts-th record; the parts meet in
+// shared memory.  The order of all sums is fixed.  Bound by three dependent rounds of loads and the launch: some 4 us
+// for 296 records of 4 rows of 128, whose 0.6 MB come from L2.
 #include "cache4.cuh"
 #include "cache4_work.cuh"
 #include "dense.cuh"

@@ -2,19 +2,25 @@
 //
 // A CTA takes 256 rows of a key/value head (new tokens times the query heads that share it) as two tiles of 128 and
 // walks over tiles of 128 positions.  Roles: three warps turn codes of keys into FP16 numbers in shared memory, rounded
-// once (l + s c, 11 bits), three those of values; one for each tile of rows issues tcgen05.mma; four for each tile of rows have a row a thread.
+// once (l + s c, 11 bits), three those of values; one for each tile of rows issues tcgen05.mma; four for each tile of
+// rows have a row a thread.
 //   S = Q K^T    both operands in shared memory, 128 FP32 columns of tensor memory for each tile of rows
 //   softmax      a thread reads its row; the weights go back over S as FP16, with a factor of 2^6 that leaves small
 //                ones their bits (the sum of the weights takes it out)
 //   O += P V     weights from tensor memory, values feature-major
 // so a tile of the cache is unpacked once for 256 rows, and one tile's products run beside the other's softmax.
 // BF16 queries become FP16 numbers times a power of two of their row.  The running maximum moves when the weights of 64
-// positions add up to more than 2^8 of its own; sums are FP32.  A position that a row does not see is masked before the maximum, and values are finite
-// (append marks a NaN in the key), so nothing behind a row's own position reaches it.
+// positions add up to more than 2^8 of its own; sums are FP32.  A position that a row does not see is masked before the
+// maximum, and values are finite (append marks a NaN in the key), so nothing behind a row's own position reaches it.
 //
 // Work: tiles of rows, longest first; or, where there are too few, all tiles of positions as one sequence of which
 // every CTA takes an equal part, parts of a tile of rows joined by a second launch in their order.
 // All mbarrier waits are bounded.
+//
+// What bounds it: 512 tokens of 32 heads of 128 over 8 behind 16000 take 158 - 172 us, 0.8 - 0.87 PFLOP/s (the power
+// limit decides); without the softmax arithmetic it would be 125, without the products 149, without the exponentials
+// 141: issue of the softmax warps and the tensor pipe, nearly level.  Heads of 64 have half the products for the same
+// softmax: nine prompts of 4200 tokens in all take 124, of which the exponentials alone are 28 at 16 a clock and SM.
 #include <type_traits>
 
 #include "cache4.cuh"
@@ -239,7 +245,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
     if (warp == 12 || warp == 13) {
         // ---------------- products of a tile of rows ----------------
         // Every value that a branch or an operand depends on is uniform by a vote or a reduction of the warp: operands then come from
-        // uniform registers (some 150 clocks an MMA otherwise).
+        // uniform registers (115 clocks an MMA, 155 otherwise).
         const int i = warp - 12;
         const bool leader = elect_one();
         const uint32_t id_s = idesc(kHalf, false), id_o = idesc(DIM, true), t0 = uniform(tmem), base = uniform(smem_u32(smem));

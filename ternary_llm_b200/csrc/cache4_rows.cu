@@ -227,7 +227,7 @@ cache4_append_kernel(const AppendArgs<T> a)
             if (!write) k.v[e] = v.v[e] = 0.f;
             bad = bad || k.v[e] != k.v[e] || v.v[e] != v.v[e];
         }
-        bad = __ballot_sync(0xffffffffu, bad) >> ((tid & 31) / kLanes * kLanes) & (kLanes == 32 ? 0xffffffffu : (1u << kLanes) - 1);
+        bad = __ballot_sync(0xffffffffu, bad) >> ((tid & 31) / kLanes * kLanes) & ((1u << kLanes) - 1);
         if (bad) {                                         // a NaN counts as 0
 #pragma unroll
             for (int e = 0; e < 8; e++) {

@@ -2,12 +2,13 @@
 //
 // A key/value head's rows (new tokens times the query heads that share it, up to 4, 8 or 16 at once) go through the
 // cache together on mma.sync.  With keys k = l + s c and values alike, scales and lowest values stay outside the products:
-//   scores   sum_groups s (c . q) + l sum q   c . q in integers: codes, or codes times 16, are bytes after one mask, a query is 16 bits of its largest entry in the group, as two signed bytes in neighbouring columns
-//            of the product (m16n8k32), whose sums are joined exactly.  Positions are the rows of the product.
+//   scores   sum_groups s (c . q) + l sum q   c . q in integers: codes, or codes times 16, are bytes after one mask, a
+//            query is 16 bits of its largest entry in the group, as two signed bytes in neighbouring columns of the
+//            product (m16n8k32), whose sums are joined exactly.  Positions are the rows of the product.
 //   outputs  sum_p (w s) (c - 8) + sum_p w (l + 8 s)   codes are FP16 numbers after a mask and an addition or
 //            multiplication for two, w s is rounded to FP16 (11 bits of it, with a power of two that follows the largest
-//            scale seen, so that small scales do not run out of exponents) and meets the difference from the middle of the
-//            group's range; the second sum is FP32.  Channels are the rows of the product (m16n8k16), columns the
+//            scale seen, so that small scales do not run out of exponents) and meets the difference from the middle of
+//            the group's range; the second sum is FP32.  Channels are the rows of the product (m16n8k16), columns the
 //            query rows, or with up to four of them the four for the first and the four for the second group.
 // Weights come out of the first product by position and go into the second as pairs of positions: movmatrix, an 8 x 8
 // transposition in registers.  The running maximum moves when a score exceeds it by more than 2^8; sums are FP32.
@@ -520,7 +521,12 @@ StepPlan step_plan(const Cache4& c, int tokens, int heads, int max_new, int max_
     // sequences of 32 heads over 8: heads of 128 behind 300 6.4 / 14.2 in one CTA, 12.1 / 17.2 cut; behind 800 8.8 / 20.1, 12.7 / 24.3; behind
     // 1200 10.3 / 24.0, 12.4 / 27.6; behind 2000 13.7 / 34.0, 11.4 / 37.5; heads of 64 behind 2000 9.3 / 21.5, 9.5 / 25.3.
     p.whole = len <= 160000 / c.dim;
-    p.ctas = p.whole ? (int)(items < 65536 ? items : 65536) : p.rows == 16 ? 148 : 296;
+    // More than two such rounds of CTAs: one round, each with an equal number of tiles in a row, which saves what a CTA does before its first
+    // tile, and costs where lengths differ.  One token each, 32 heads of 128 over 8, up to 800 positions, us, one round / a CTA a tile: equal
+    // lengths 48 sequences 22.2 / 20.4, 96 33.7 / 36.2, 256 76.9 / 97.9; lengths between 1 and that 20.5 / 16.6, 30.0 / 27.6, 69.5 / 77.3;
+    // 1024 of 8 heads over one 59 / 91.
+    const int round = p.rows == 16 ? 148 : 296;
+    p.ctas = p.whole && items <= 2 * round ? (int)items : round;
     p.bytes = p.whole ? 0 : join_bytes(c.dim, p.rows, p.ctas);
     return p;
 }

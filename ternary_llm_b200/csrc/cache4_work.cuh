@@ -85,6 +85,7 @@ struct Work {
     {
         Span none;
         none.row0 = none.n = none.len = 0;
+        none.falls = false;
         return i < s.batch ? span_of(s, i, false) : none;
     }
     static __device__ __forceinline__ int scan(int v, int lane)
@@ -123,12 +124,15 @@ struct Work {
     {
         int total = 0, mine = 0;                      // mine: units of a head of the lane's sequence, of the last 32
         Span sp;
+        bool falls = false;                           // then nothing is done: the units of such a call may not fit
         for (int b0 = 0; b0 < s.batch; b0 += 32) {
             sp = lane_span(b0 + lane);
+            falls = falls || sp.falls;
             if (c == 0 && b0 + lane < s.batch) span_of(s, b0 + lane, true);
             mine = units(sp, lane);
             total += __reduce_add_sync(0xffffffffu, mine * kv_heads);
         }
+        if (__any_sync(0xffffffffu, falls)) total = 0;
         Start r;
         r.share = max((total + parts - 1) / parts, whole ? 1 : kLeast);
         r.x = min((long long)c * r.share, (long long)total);
@@ -209,11 +213,11 @@ struct Work {
         set_tile(0);
     }
 };
-// Whether the units of a call fit 31 bits, whatever first and lens hold (even all rows in every sequence).
-inline bool work_fits(const Cache4& c, int tokens, int heads, int rows, int chunk)
+// Whether the units of a call fit 31 bits, whatever lens and a rising first hold.
+inline bool work_fits(const Cache4Call& a, int rows, int chunk)
 {
-    const double tiles = (double)tokens * (heads / c.kv_heads) / rows + 1, units = (double)c.rows / chunk + 22;
-    return tiles * units * c.batch * c.kv_heads < 2e9;
+    const double tiles = (double)a.s.tokens * (a.heads / a.c.kv_heads) / rows + a.c.batch, units = (double)a.s.rows / chunk + 22;
+    return tiles * units * a.c.kv_heads < 2e9;
 }
 
 template <typename T> struct Pair2;

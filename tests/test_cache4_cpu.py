@@ -1,5 +1,6 @@
 """Host side of the 4-bit cache: frequencies and turns of rotary positions against exact arithmetic, the layout's helpers, refusals that need
 no GPU."""
+import copy
 import ctypes
 import math
 from fractions import Fraction
@@ -216,3 +217,34 @@ def test_shapes_refused_in_python():
         ops.rotary(x, None, torch.zeros(3, dtype=torch.int32), t, k_out=x)
     with pytest.raises(ValueError, match="behind one another"):
         ops._rows(x.transpose(0, 1), torch.float16, "q", 2, 3, 64)
+
+
+def test_outputs_may_not_lie_over_other_inputs():
+    h = tl.lib()
+    three = ctypes.byref(_lib.RotaryTableDesc(P, 64, 1, 1.0))
+
+    def rotary(q, qo, k, ko):
+        refused(SHAPE, h.tllm_b200_rotary, 0, three, P, 3, q, qo, 2, k, ko, 1, 64, 0)
+
+    rotary(heads(P), heads(P * 2), heads(P * 2), heads(P * 2))                     # q_out over k
+    rotary(heads(P), heads(P), heads(P * 2, 64), heads(P, 64))                     # k_out over q
+    rotary(heads(P), heads(P * 2), heads(P * 4, 64), heads(P * 2 + 256, 64))       # k_out over q_out
+    rotary(heads(P, 192), heads(P, 192), heads(P + 128, 192), heads(P + 128, 192))  # rows of 192, keys begin inside the queries' 256 bytes
+    c = cache()
+    refused(SHAPE, h.tllm_b200_cache4_append, ctypes.byref(c), 0, None, P, P, 3, heads(P), heads(P * 2), 2, heads(P * 2), heads(P * 4))
+    refused(SHAPE, h.tllm_b200_cache4_append, ctypes.byref(c), 0, None, P, P, 3, heads(P), heads(P * 2), 2, heads(P * 4), heads(P * 2 + 16))
+    refused(SHAPE, h.tllm_b200_cache4_read, ctypes.byref(c), 0, P, P, 3, heads(P), heads(P + 16))
+    refused(SHAPE, h.tllm_b200_rotary, 0, three, P, 2 ** 31 - 1, heads(), heads(), 2, None, None, 0, 64, 0)
+
+
+def test_tensors_of_a_cache_and_a_table_are_set_once():
+    kc, kp = torch.zeros(1, 1, 8, 32, dtype=torch.uint8), torch.zeros(1, 1, 8, 1, 2, dtype=torch.float16)
+    c, t = ops.Cache4(kc, kp, kc.clone(), kp.clone()), ops.RotaryTable(64, 500000.0, half=False, scaling=dict(type="linear", factor=2.0), amplitude=1.5, device="cpu")
+    for o, name, value in ((c, "k_codes", kc.clone()), (c, "rows", 4), (t, "turns", t.turns.clone()), (t, "amplitude", 1.0)):
+        with pytest.raises(AttributeError, match="make another"):
+            setattr(o, name, value)
+    d, u = copy.deepcopy(c), copy.deepcopy(t)
+    assert d.k_codes.data_ptr() != c.k_codes.data_ptr() and torch.equal(d.k_codes, c.k_codes) and d.rows == 8
+    assert u.turns.data_ptr() != t.turns.data_ptr() and torch.equal(u.turns, t.turns)
+    assert (u.rot_dim, u.half, u.amplitude, u.frequencies) == (64, False, 1.5, t.frequencies)
+    assert copy.copy(c).k_codes is c.k_codes

@@ -575,3 +575,28 @@ def test_refusals_on_the_device():
         ops.rotary(x, None, ints(1, 2), ops.RotaryTable(64))
     with pytest.raises(tl.TllmError, match="16-byte"):
         ops.rotary(torch.zeros(3 * 128 + 1, dtype=torch.float16, device="cuda")[1:].view(3, 2, 64), None, ints(1, 2, 3), ops.RotaryTable(64))
+
+
+def test_very_many_short_sequences():
+    n = 32768
+    attention_case(torch.float16, [i % 4 for i in range(n)], [1] * n, 1, 1, 64, rows=64, sequences={0, 1, 2, 3, 31, 32, 1000, n - 1})
+
+
+@pytest.mark.parametrize("heads,new", [(8, 1), (64, 1), (64, 2)])
+def test_more_tiles_than_ctas(heads, new):
+    """A CTA takes several tiles, of different sequences."""
+    n = 90
+    attention_case(torch.bfloat16, [(7 * i) % 93 * (i % 5 > 0) for i in range(n)], [new * (i % 7 != 2) for i in range(n)], heads, 8, 64, sequences=set(range(0, n, 5)))
+
+
+def test_a_copy_of_a_cache_is_its_own():
+    import copy
+    c = new_cache(1, 1, 8, 64)
+    d = copy.deepcopy(c)
+    was = contents(c)
+    x = torch.randn(4, 1, 64, device="cuda").half()
+    ops.append(d, None, x, x, ints(0, 4), ints(4))
+    k = torch.empty_like(x)
+    ops.read(d, k, None, ints(0, 4), ints(4))
+    tl.check_device_errors()
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(contents(c), was)) and (k.float() - x.float()).abs().max() < 0.5
