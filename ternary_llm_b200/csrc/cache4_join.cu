@@ -109,7 +109,8 @@ int launch_cache4_join(const Cache4Call& a, Rows<T> out, int rows, int ctas, cud
     if (rows == 4) return launch<T, 4>(a, out, ctas, stream);
     if (rows == 8) return launch<T, 8>(a, out, ctas, stream);
     if (rows == 16) return launch<T, 16>(a, out, ctas, stream);
-    return launch<T, kPromptRows>(a, out, ctas, stream);
+    if (rows == 128) return launch<T, 128>(a, out, ctas, stream);
+    return launch<T, 256>(a, out, ctas, stream);
 }
 
 template int launch_cache4_join<half>(const Cache4Call&, Rows<half>, int, int, cudaStream_t);

@@ -1,7 +1,7 @@
 // Attention over the 4-bit key/value cache for many rows a sequence, on the 5th-generation tensor cores.
 //
-// A CTA takes 256 rows of a key/value head (new tokens times the query heads that share it) as two tiles of 128 and
-// walks over tiles of 128 positions.  Roles: three warps turn codes of keys into FP16 numbers in shared memory, rounded
+// A CTA takes 256 rows of a key/value head (new tokens times the query heads that share it) as two tiles of 128, or one
+// tile of 128 where there are SMs for it, and walks over tiles of 128 positions.  Roles: three warps turn codes of keys into FP16 numbers in shared memory, rounded
 // once (l + s c, 11 bits), three those of values; one for each tile of rows issues tcgen05.mma; four for each tile of
 // rows have a row a thread.
 //   S = Q K^T    both operands in shared memory, 128 FP32 columns of tensor memory for each tile of rows
@@ -21,6 +21,7 @@
 // limit decides); without the softmax arithmetic it would be 125, without the products 149, without the exponentials
 // 141: issue of the softmax warps and the tensor pipe, nearly level.  Heads of 64 have half the products for the same
 // softmax: nine prompts of 4200 tokens in all take 124, of which the exponentials alone are 28 at 16 a clock and SM.
+#include <cmath>
 #include <type_traits>
 
 #include "cache4.cuh"
@@ -36,21 +37,22 @@ namespace {
 
 using namespace gemm;
 
-constexpr int kTile = kPromptChunk, kRows = kPromptRows, kRowTiles = kRows / kTile;
+constexpr int kTile = kPromptChunk;
 constexpr int kThreads = 512;                        // warps: softmax of a tile of rows 0-3, of the other 4-7, its products 12, 13, keys and values the rest
 constexpr int kUnpackThreads = 96;                   // of keys, and of values
 constexpr int kBlock = kTile * 128;                  // bytes of 64 columns of a tile: 128-byte rows
 constexpr int kStages = 2, kHalf = kTile / 2;
 constexpr float kLift = 6.f, kMost = 16384.f, kLog2e = 1.4426950408889634f;          // kMost: 2^8 times what kLift lifts
 
-template <int DIM>
+template <int DIM, int ROW_TILES>
 struct Prompt {
+    static constexpr int kRows = ROW_TILES * kTile;
     static constexpr int kBlocks = DIM / 64;
     static constexpr int kOperand = kBlocks * kBlock;                              // bytes of a tile
     static constexpr int kRounds = (DIM / 32 * kTile + kUnpackThreads - 1) / kUnpackThreads;      // of 16 bytes a thread, of keys or values
     static constexpr int kRawSide = kRounds * kUnpackThreads * 20;                                // the next tile's codes and params
-    static constexpr int kSmem = (kRowTiles + 2 * kStages) * kOperand + 2 * kRawSide + 1024;
-    static constexpr uint32_t kTmemCols = kRowTiles * (kTile + DIM) <= 384 && kRowTiles * (kTile + DIM) > 256 ? 512 : kRowTiles * (kTile + DIM);
+    static constexpr int kSmem = (ROW_TILES + 2 * kStages) * kOperand + 2 * kRawSide + 1024;
+    static constexpr uint32_t kTmemCols = ROW_TILES == 2 ? 512 : 256;                // a power of two that holds ROW_TILES (kTile + DIM)
 };
 
 __device__ __forceinline__ uint32_t idesc(int n, bool feature_major)
@@ -126,9 +128,13 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 
 // A tile's rows of a key/value head and the tiles of positions [j0, j1) of its `chunks`, one after the other for this CTA;
 // every role walks over the same.
-struct Walk : Work<kRows, kTile> {
+template <int ROWS>
+struct Walk : Work<ROWS, kTile> {
+    using Base = Work<ROWS, kTile>;
+    using Base::s, Base::per, Base::kv_heads, Base::whole, Base::x, Base::to, Base::b, Base::head, Base::tile, Base::offset, Base::rows, Base::chunks,
+        Base::span, Base::kFixed, Base::chunk_at;
     int from_top, step, j0, j1, segment;
-    __device__ __forceinline__ Walk(const Cache4Call& a, bool whole_, const Start& f) : Work(a.s, a.heads / a.c.kv_heads, a.c.kv_heads, whole_), segment(-1)
+    __device__ __forceinline__ Walk(const Cache4Call& a, bool whole_, const typename Base::Start& f) : Base(a.s, a.heads / a.c.kv_heads, a.c.kv_heads, whole_), segment(-1)
     {
         if (whole) {
             const int pairs = s.batch * kv_heads, pair = blockIdx.x % pairs;
@@ -139,7 +145,7 @@ struct Walk : Work<kRows, kTile> {
             span = span_of(s, b, blockIdx.x / pairs == 0 && head == 0 && threadIdx.x == 0);
             rows = span.n * per;
         } else {
-            begin(f);
+            Base::begin(f);
         }
     }
     __device__ __forceinline__ bool advance()
@@ -147,16 +153,16 @@ struct Walk : Work<kRows, kTile> {
         if (whole) {
             segment++;
             from_top += step;
-            const int tl = (rows + kRows - 1) / kRows - 1 - from_top;
+            const int tl = (rows + ROWS - 1) / ROWS - 1 - from_top;
             if (tl < 0) return false;
-            set_tile(tl);
+            Base::set_tile(tl);
             j0 = 0;
             j1 = chunks;
             return true;
         }
         do {
             if (x >= to) return false;
-            if (++segment > 0) next();
+            if (++segment > 0) Base::next();
             j0 = chunk_at(offset);
             j1 = chunk_at(min(kFixed + chunks, offset + (to - x)));
             x += kFixed + chunks - offset;
@@ -164,7 +170,7 @@ struct Walk : Work<kRows, kTile> {
         return true;
     }
     __device__ __forceinline__ bool complete() const { return j0 == 0 && j1 == chunks; }
-    __device__ __forceinline__ int tile_rows(int i) const { return min(kTile, rows - tile * kRows - i * kTile); }
+    __device__ __forceinline__ int tile_rows(int i) const { return min(kTile, rows - tile * ROWS - i * kTile); }
 };
 
 // the last three by tile of rows and half of a tile of positions
@@ -199,22 +205,24 @@ __device__ __forceinline__ void unpack32(uint32_t dst, uint32_t turn, const uint
     }
 }
 
-template <typename T, int DIM>
+template <typename T, int DIM, int ROW_TILES>
 __global__ void __launch_bounds__(kThreads, 1)
 cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out, const bool whole)
 {
-    using P = Prompt<DIM>;
+    using P = Prompt<DIM, ROW_TILES>;
+    using W = Walk<P::kRows>;
+    constexpr int kRows = P::kRows;
     constexpr int kCodes = DIM / 32;                                       // 16-byte pieces of a row of codes
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) uint64_t bars[kBars];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
-    __shared__ Walk::Start start;
+    __shared__ typename W::Base::Start start;
     __shared__ float row_scale[kRows];
     pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    uint8_t *qs = smem, *ks = qs + kRowTiles * P::kOperand, *vs = ks + kStages * P::kOperand, *raw = vs + kStages * P::kOperand;
+    uint8_t *qs = smem, *ks = qs + ROW_TILES * P::kOperand, *vs = ks + kStages * P::kOperand, *raw = vs + kStages * P::kOperand;
     const uint32_t bar0 = smem_u32(bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
     volatile int* abortp = &abort_flag;
@@ -224,7 +232,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
         for (int i = 0; i < kBars; i++) {
             const int pair = i & ~1;
             mbar_init(bar(i), pair == kQFull || (i >= kPReady && i < kLast) ? kTile : pair == kKFull || pair == kVFull ? kUnpackThreads :
-                              pair == kKEmpty || pair == kVEmpty ? kRowTiles : 1);
+                              pair == kKEmpty || pair == kVEmpty ? ROW_TILES : 1);
         }
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -235,14 +243,14 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pdl_wait();
-    if (warp == 13 && !whole) Walk::Work(a.s, a.heads / a.c.kv_heads, a.c.kv_heads, false).find(blockIdx.x, gridDim.x, lane, &start);
+    if (warp == 13 && !whole) typename W::Base(a.s, a.heads / a.c.kv_heads, a.c.kv_heads, false).find(blockIdx.x, gridDim.x, lane, &start);
     if (!whole && tid == 0) entry_of(a.ws, blockIdx.x)->parts = 0;
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot;                                       // S of both tiles of rows, then O of both
 
-    if (warp == 12 || warp == 13) {
+    if (warp >= 12 && warp < 12 + ROW_TILES) {
         // ---------------- products of a tile of rows ----------------
         // Every value that a branch or an operand depends on is uniform by a vote or a reduction of the warp: operands then come from
         // uniform registers (115 clocks an MMA, 155 otherwise).
@@ -250,11 +258,11 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
         const bool leader = elect_one();
         const uint32_t id_s = idesc(kHalf, false), id_o = idesc(DIM, true), t0 = uniform(tmem), base = uniform(smem_u32(smem));
         const uint64_t qd = make_sw128_desc(base + i * P::kOperand);
-        const uint32_t to_s = t0 + i * kTile, to_o = t0 + kRowTiles * kTile + i * DIM;
+        const uint32_t to_s = t0 + i * kTile, to_o = t0 + ROW_TILES * kTile + i * DIM;
         const auto wait = [&](int k, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar(k), parity, abortp)) != 0; };
         // half h of a tile of positions
         const auto score = [&](int h, uint32_t st) {
-            const uint64_t kd = make_sw128_desc(base + (kRowTiles + st) * P::kOperand) + h * (kHalf * 128 >> 4);
+            const uint64_t kd = make_sw128_desc(base + (ROW_TILES + st) * P::kOperand) + h * (kHalf * 128 >> 4);
             fence_after();
 #pragma unroll
             for (int j = 0; j < P::kBlocks; j++)
@@ -266,13 +274,13 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
             commit(leader, bar(kSFull + i + 2 * h));
         };
         const auto output = [&](int h, uint32_t st, bool first) {
-            const uint64_t vd = feature_major_desc(base + (kRowTiles + kStages + st) * P::kOperand) + h * (kHalf * 128 >> 4);
+            const uint64_t vd = feature_major_desc(base + (ROW_TILES + kStages + st) * P::kOperand) + h * (kHalf * 128 >> 4);
             fence_after();
 #pragma unroll
             for (int k = 0; k < kHalf / 16; k++) mma_ts(leader, to_o, to_s + h * kHalf + k * 8, vd + k * (2048 >> 4), id_o, !first || k > 0);
             commit(leader, bar(kPvDone + i + 2 * h));
         };
-        Walk w(a, whole, start);
+        W w(a, whole, start);
         uint32_t n = 0, items = 0, rounds = 0;                             // tiles of positions so far; with rows here: segments, tiles
         bool ok = true;
         while (ok && __any_sync(0xffffffffu, w.advance())) {
@@ -320,7 +328,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
             __syncwarp();
             mbar_wait(bar(kLast + i), 0, &never);
         }
-    } else if (warp >= 8) {
+    } else if (warp >= 8 && warp != 13) {
         // ---------------- unpacking: 16 bytes of a position at once ----------------
         // A thread copies what it unpacks for the tile after this one (cp.async), and reads it back itself.
         // Three warps for keys and three for values, so that neither waits for the other's stage.  Piece e is piece e / 128 of row e % 128; the
@@ -333,7 +341,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
         const int full = values ? kVFull : kKFull, empty = values ? kVEmpty : kKEmpty;
         const uint8_t* codes = values ? a.c.vc : a.c.kc;
         const half2* params = values ? a.c.vp : a.c.kp;
-        Walk w(a, whole, start);
+        W w(a, whole, start);
         uint32_t n = 0;
         bool ok = true;
         while (ok && w.advance()) {
@@ -376,11 +384,11 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
             asm volatile("cp.async.wait_all;" ::: "memory");
         }
         if (!ok) abort_flag = 1;
-    } else {
+    } else if (warp < 4 * ROW_TILES) {
         // ---------------- softmax: a row a thread ----------------
         const int i = warp >> 2, row = tid & (kTile - 1);
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, row_s = tmem + i * kTile + lanes, row_o = tmem + kRowTiles * kTile + i * DIM + lanes;
-        Walk w(a, whole, start);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, row_s = tmem + i * kTile + lanes, row_o = tmem + ROW_TILES * kTile + i * DIM + lanes;
+        W w(a, whole, start);
         const bool wide = ((reinterpret_cast<uintptr_t>(out.p) | (uintptr_t)out.ld * sizeof(T)) & 31) == 0;     // outputs on whole sectors
         uint32_t rounds = 0;
         bool ok = true;
@@ -563,20 +571,20 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
     }
 }
 
-template <typename T, int DIM>
+template <typename T, int DIM, int ROW_TILES>
 int launch(const Cache4Call& a, Rows<const T> q, Rows<T> out, const PromptPlan& p, cudaStream_t stream)
 {
     static bool attr[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return fail(TLLM_ERR_LAUNCH, "cache4_prompt: no current device");
-    const auto kernel = cache4_prompt_kernel<T, DIM>;
+    const auto kernel = cache4_prompt_kernel<T, DIM, ROW_TILES>;
     if (!attr[dev]) {
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<DIM>::kSmem);
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<DIM, ROW_TILES>::kSmem);
         attr[dev] = true;
     }
-    const int st = launch_pdl("cache4_prompt", kernel, dim3(p.ctas), dim3(kThreads), Prompt<DIM>::kSmem, stream, a, q, out, p.whole);
-    return st || p.whole ? st : launch_cache4_join<T>(a, out, kRows, p.ctas, stream);
+    const int st = launch_pdl("cache4_prompt", kernel, dim3(p.ctas), dim3(kThreads), Prompt<DIM, ROW_TILES>::kSmem, stream, a, q, out, p.whole);
+    return st || p.whole ? st : launch_cache4_join<T>(a, out, p.rows, p.ctas, stream);
 }
 
 }  // namespace
@@ -584,26 +592,48 @@ int launch(const Cache4Call& a, Rows<const T> q, Rows<T> out, const PromptPlan& 
 PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int max_len)
 {
     PromptPlan p;
-    const int per = heads / c.kv_heads, most = max_new > 0 && max_new < tokens ? max_new : tokens;
-    const long long tiles = ((long long)most * per + kRows - 1) / kRows, pairs = (long long)c.batch * c.kv_heads;
-    const long long grid = tiles * pairs < (1 << 20) ? tiles * pairs : (1 << 20) / pairs * pairs;
-    // A tile of rows stays in one CTA unless the longest would keep its SM busy for more than seven tiles of positions (some 2 us each) after
-    // the others are done, which is what cutting costs in records and a second launch.  Both ways, us, 32 heads over 8: of 128, a prompt of 1500
-    // 39 whole, 57 cut, 2000 52 / 74; of 64, four prompts of 700 38 / 51; 512 tokens behind 16000 are 64 tiles of rows of 129 tiles each,
-    // which whole would take twice the 158 us.
-    const int len = max_len > 0 && max_len < c.rows ? max_len : c.rows;
+    const int per = heads / c.kv_heads, most = max_new > 0 && max_new < tokens ? max_new : tokens, len = max_len > 0 && max_len < c.rows ? max_len : c.rows;
     const double longest = (len + kTile - 1) / kTile, mean = longest - (most < len ? most : len) / (2.0 * kTile);
-    const double rows = (double)tokens * per / kRows > (double)c.batch ? (double)tokens * per / kRows : (double)c.batch;
-    p.whole = longest - rows * c.kv_heads * mean / 148 <= 7;
+    // Tiles of `rows` rows, where every sequence has as many rows as it may.
+    const auto tiles_of = [&](int rows) {
+        const double by_tokens = (double)tokens * per / rows + c.batch, by_most = (double)c.batch * (((long long)most * per + rows - 1) / rows);
+        return (by_tokens < by_most ? by_tokens : by_most) * c.kv_heads;
+    };
+    if (tiles_of(128) <= 148) {
+        // An SM for each tile of 128 rows: the quickest of these tiles whole, cut, and tiles of 256 rows cut, as they measure, us: 8 + 1.9 for each
+        // tile of positions, or 19 + 1.85 for each that a CTA takes, or 27 + 2.35; sequences of a batch differ, so that cut ones have fewer.
+        // 32 heads of 128 over 8, one sequence: 79 tokens behind 500 18.6 / 25.0 / 25.9, behind 2500 50.1 / 27.3 / 35.7, behind 16000 243 / 64 /
+        // 61; 500 behind 1200 36.4 / 48.2 / 42.0, behind 6000 111 / 117 / 85.  Tiles of 256 whole take 22.0, 60.9, 297, 42.8 and 131.
+        const double few = c.batch > 1 ? 0.85 : 1;
+        const auto cut = [&](int rows) { return fmax(tiles_of(rows) * (few * mean + Work<128, kTile>::kFixed) / 148, (double)Work<128, kTile>::kLeast); };
+        const double whole = 8 + 1.9 * longest, halves = 19 + 1.85 * cut(128), full = 27 + 2.35 * cut(256);
+        p.rows = full < fmin(whole, halves) ? 256 : 128;
+        p.whole = whole <= fmin(halves, full);
+    } else {
+        // A tile of rows stays in one CTA unless the longest would keep its SM busy for more than seven tiles of positions (some 2 us each) after
+        // the others are done, which is what cutting costs in records and a second launch.  Both ways, us, 32 heads over 8: of 128, a prompt of
+        // 1500 39 whole, 57 cut, 2000 52 / 74; of 64, four prompts of 700 38 / 51.
+        const double rows = (double)tokens * per / 256 > (double)c.batch ? (double)tokens * per / 256 : (double)c.batch;
+        p.rows = 256;
+        p.whole = longest - rows * c.kv_heads * mean / 148 <= 7;
+    }
+    const long long tiles = ((long long)most * per + p.rows - 1) / p.rows, pairs = (long long)c.batch * c.kv_heads;
+    const long long grid = tiles * pairs < (1 << 20) ? tiles * pairs : (1 << 20) / pairs * pairs;
     p.ctas = p.whole ? (int)(grid < pairs ? pairs : grid) : 148;
-    p.bytes = p.whole ? 0 : join_bytes(c.dim, kRows, p.ctas);
+    p.bytes = p.whole ? 0 : join_bytes(c.dim, p.rows, p.ctas);
     return p;
+}
+
+template <typename T, int DIM>
+static int launch_rows(const Cache4Call& a, Rows<const T> q, Rows<T> out, const PromptPlan& p, cudaStream_t stream)
+{
+    return p.rows == kTile ? launch<T, DIM, 1>(a, q, out, p, stream) : launch<T, DIM, 2>(a, q, out, p, stream);
 }
 
 template <typename T>
 int launch_cache4_prompt(const Cache4Call& a, Rows<const T> q, Rows<T> out, const PromptPlan& p, cudaStream_t stream)
 {
-    return a.c.dim == 64 ? launch<T, 64>(a, q, out, p, stream) : launch<T, 128>(a, q, out, p, stream);
+    return a.c.dim == 64 ? launch_rows<T, 64>(a, q, out, p, stream) : launch_rows<T, 128>(a, q, out, p, stream);
 }
 
 template int launch_cache4_prompt<half>(const Cache4Call&, Rows<const half>, Rows<half>, const PromptPlan&, cudaStream_t);

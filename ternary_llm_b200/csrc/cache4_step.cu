@@ -520,7 +520,7 @@ StepPlan step_plan(const Cache4& c, int tokens, int heads, int max_new, int max_
     // A tile's positions stay in one CTA while that takes no longer than a second launch and what it waits for.  Both ways, us, one / 48
     // sequences of 32 heads over 8: heads of 128 behind 300 6.4 / 14.2 in one CTA, 12.1 / 17.2 cut; behind 800 8.8 / 20.1, 12.7 / 24.3; behind
     // 1200 10.3 / 24.0, 12.4 / 27.6; behind 2000 13.7 / 34.0, 11.4 / 37.5; heads of 64 behind 2000 9.3 / 21.5, 9.5 / 25.3.
-    p.whole = len <= 160000 / c.dim;
+    p.whole = len <= kStepWhole / c.dim;
     // More than two such rounds of CTAs: one round, each with an equal number of tiles in a row, which saves what a CTA does before its first
     // tile, and costs where lengths differ.  One token each, 32 heads of 128 over 8, up to 800 positions, us, one round / a CTA a tile: equal
     // lengths 48 sequences 22.2 / 20.4, 96 33.7 / 36.2, 256 76.9 / 97.9; lengths between 1 and that 20.5 / 16.6, 30.0 / 27.6, 69.5 / 77.3;

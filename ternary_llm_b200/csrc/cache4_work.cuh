@@ -7,7 +7,8 @@
 namespace tllm {
 
 constexpr int kStepChunk = 32;                       // positions a warp of cache4_step.cu takes at once
-constexpr int kPromptChunk = 128, kPromptRows = 256; // positions and rows a CTA of cache4_prompt.cu takes at once
+constexpr int kStepWhole = 160000;                   // entries of a head's positions up to which one CTA takes a tile of them, see step_plan
+constexpr int kPromptChunk = 128;                    // positions a CTA of cache4_prompt.cu takes at once
 // Floats of the part of a tile's rows that one CTA found: maxima, sums, outputs.
 template <int DIM, int ROWS> constexpr int kRecord = ROWS * (DIM + 2);
 
@@ -38,6 +39,7 @@ template <typename T>
 int launch_cache4_step(const Cache4Call& a, Rows<const T> q, Rows<T> out, const StepPlan& p, cudaStream_t stream);
 
 struct PromptPlan {
+    int rows;                                        // of a CTA: 128 or 256
     bool whole;
     int ctas;
     size_t bytes;
@@ -59,7 +61,7 @@ int launch_cache4_join(const Cache4Call& a, Rows<T> out, int rows, int ctas, cud
 template <int R, int CHUNK>
 struct Work {
     static constexpr int kFixed = CHUNK == kStepChunk ? 20 : 4;
-    static constexpr int kLeast = CHUNK == kStepChunk ? 36 : 6;            // units that a CTA takes at least where work is cut
+    static constexpr int kLeast = CHUNK == kStepChunk ? 36 : 4;            // units that a CTA takes at least where work is cut
     struct Start {
         int x, to, share, b, head, tile, offset;
     };

@@ -47,10 +47,11 @@ def rotate(x, positions, frequencies, amplitude, half):
 
 
 def attention(q, k, v, position, scale, v_size):
-    """One head: q [n, dim] at `position` [n], k and v [m, dim].  (result, sum of weights times v_size, largest sum of |q k| scale)."""
+    """One head: q [n, dim] at `position` [n], k and v [m, dim].  (result, sum of weights times v_size, largest sum of |q k scale|): a
+    score is a sum of dim terms of these sizes, whatever the sign of the scale, and roundings are in proportion to them."""
     s = q @ k.T * scale
     sees = np.arange(len(k))[None] <= position[:, None]
-    reach = np.where(sees, np.abs(q) @ np.abs(k).T * scale, 0).max(-1, initial=0.0)
+    reach = np.where(sees, np.abs(q) @ np.abs(k).T * abs(scale), 0).max(-1, initial=0.0)
     s = np.where(sees, s, -np.inf)
     top = s.max(-1, initial=-np.inf, keepdims=True)
     p = np.where(sees, np.exp(s - np.where(np.isfinite(top), top, 0)), 0)

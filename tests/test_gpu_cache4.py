@@ -589,6 +589,15 @@ def test_more_tiles_than_ctas(heads, new):
     attention_case(torch.bfloat16, [(7 * i) % 93 * (i % 5 > 0) for i in range(n)], [new * (i % 7 != 2) for i in range(n)], heads, 8, 64, sequences=set(range(0, n, 5)))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("before,new,heads,kv_heads,dim", [
+    ([0], [79], 32, 8, 128), ([700], [150], 24, 24, 64), ([2100], [79], 32, 8, 128), ([5000, 40], [33, 100], 16, 4, 64), ([9000], [129], 16, 2, 128), ([3000], [500], 8, 4, 128),
+    ([130] * 5, [200, 0, 128, 1, 65], 8, 2, 64), ([6000], [600], 32, 8, 64)])
+def test_prompts_with_an_sm_for_each_tile(dtype, before, new, heads, kv_heads, dim):
+    attention_case(dtype, before, new, heads, kv_heads, dim, sequences={0, 1, 4})
+    attention_case(dtype, before, new, heads, kv_heads, dim, scale=-0.2, hints=False, wide=24, sequences={0, 3})
+
+
 def test_a_copy_of_a_cache_is_its_own():
     import copy
     c = new_cache(1, 1, 8, 64)
