@@ -20,7 +20,7 @@
 // What bounds it: 512 tokens of 32 heads of 128 over 8 behind 16000 take 158 - 172 us, 0.8 - 0.87 PFLOP/s (the power
 // limit decides); without the softmax arithmetic it would be 125, without the products 149, without the exponentials
 // 141: issue of the softmax warps and the tensor pipe, nearly level.  Heads of 64 have half the products for the same
-// softmax: nine prompts of 4200 tokens in all take 124, of which the exponentials alone are 28 at 16 a clock and SM.
+// softmax: nine prompts of 4529 tokens in all take 124, of which the exponentials alone are 28 at 16 a clock and SM.
 #include <cmath>
 #include <type_traits>
 
