@@ -4,7 +4,8 @@
 // tile of 128 where there are SMs for it, and walks over tiles of 128 positions.  Roles: three warps turn codes of keys into FP16 numbers in shared memory, rounded
 // once (l + s c, 11 bits), three those of values; one for each tile of rows issues tcgen05.mma; four for each tile of
 // rows have a row a thread.
-//   S = Q K^T    both operands in shared memory, 128 FP32 columns of tensor memory for each tile of rows
+//   S = Q K^T    128 FP32 columns of tensor memory for each tile of rows; keys in shared memory, queries too, or for heads
+//                of 64, where it has room, in tensor memory (nine prompts 119.7 us, 123.2 otherwise)
 //   softmax      a thread reads its row; the weights go back over S as FP16, with a factor of 2^6 that leaves small
 //                ones their bits (the sum of the weights takes it out)
 //   O += P V     weights from tensor memory, values feature-major
@@ -20,7 +21,7 @@
 // What bounds it: 512 tokens of 32 heads of 128 over 8 behind 16000 take 158 - 172 us, 0.8 - 0.87 PFLOP/s (the power
 // limit decides); without the softmax arithmetic it would be 125, without the products 149, without the exponentials
 // 141: issue of the softmax warps and the tensor pipe, nearly level.  Heads of 64 have half the products for the same
-// softmax: nine prompts of 4529 tokens in all take 124, of which the exponentials alone are 28 at 16 a clock and SM.
+// softmax: nine prompts of 4529 tokens in all take 120, of which the exponentials alone are 28 at 16 a clock and SM.
 #include <cmath>
 #include <type_traits>
 
@@ -52,7 +53,8 @@ struct Prompt {
     static constexpr int kRounds = (DIM / 32 * kTile + kUnpackThreads - 1) / kUnpackThreads;      // of 16 bytes a thread, of keys or values
     static constexpr int kRawSide = kRounds * kUnpackThreads * 20;                                // the next tile's codes and params
     static constexpr int kSmem = (ROW_TILES + 2 * kStages) * kOperand + 2 * kRawSide + 1024;
-    static constexpr uint32_t kTmemCols = ROW_TILES == 2 ? 512 : 256;                // a power of two that holds ROW_TILES (kTile + DIM)
+    static constexpr int kQueryCols = DIM == 64 ? DIM / 2 : 0;                     // of tensor memory for a tile's queries, where there is room
+    static constexpr uint32_t kTmemCols = ROW_TILES == 2 ? 512 : 256;                // a power of two that holds ROW_TILES (kTile + DIM + kQueryCols)
 };
 
 __device__ __forceinline__ uint32_t idesc(int n, bool feature_major)
@@ -258,7 +260,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
         const bool leader = elect_one();
         const uint32_t id_s = idesc(kHalf, false), id_o = idesc(DIM, true), t0 = uniform(tmem), base = uniform(smem_u32(smem));
         const uint64_t qd = make_sw128_desc(base + i * P::kOperand);
-        const uint32_t to_s = t0 + i * kTile, to_o = t0 + ROW_TILES * kTile + i * DIM;
+        const uint32_t to_s = t0 + i * kTile, to_o = t0 + ROW_TILES * kTile + i * DIM, to_q = t0 + ROW_TILES * (kTile + DIM) + i * P::kQueryCols;
         const auto wait = [&](int k, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar(k), parity, abortp)) != 0; };
         // half h of a tile of positions
         const auto score = [&](int h, uint32_t st) {
@@ -269,7 +271,8 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const uint32_t o = j * (kBlock >> 4) + k * 2;
-                    mma_ss(leader, to_s + h * kHalf, qd + o, kd + o, id_s, j > 0 || k > 0);
+                    if constexpr (P::kQueryCols > 0) mma_ts(leader, to_s + h * kHalf, to_q + k * 8, kd + o, id_s, k > 0);
+                    else mma_ss(leader, to_s + h * kHalf, qd + o, kd + o, id_s, j > 0 || k > 0);
                 }
             commit(leader, bar(kSFull + i + 2 * h));
         };
@@ -436,7 +439,20 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
                     *reinterpret_cast<uint4*>(piece(k)) = make_uint4(x[0], x[1], x[2], x[3]);
                 }
             }
-            fence_async();
+            if constexpr (P::kQueryCols > 0) {
+                __syncwarp();
+                uint32_t x[32];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(qs + i * P::kOperand + row * 128 + ((e ^ (row & 7)) << 4));
+                    x[4 * e] = v.x, x[4 * e + 1] = v.y, x[4 * e + 2] = v.z, x[4 * e + 3] = v.w;
+                }
+                tmem_st32(tmem + ROW_TILES * (kTile + DIM) + i * P::kQueryCols + lanes, x);
+                wait_st();
+                fence_before();
+            } else {
+                fence_async();
+            }
             __syncwarp();
             mbar_arrive(bar(kQFull + i));
             float scale2 = fabsf(a.scale) * kLog2e;
