@@ -5,23 +5,23 @@
 // once (l + s c, 11 bits), three those of values; one for each tile of rows issues tcgen05.mma; four for each tile of
 // rows have a row a thread.
 //   S = Q K^T    128 FP32 columns of tensor memory for each tile of rows; keys in shared memory, queries too, or for heads
-//                of 64, where it has room, in tensor memory (nine prompts 119.7 us, 123.2 otherwise)
+//                of 64, where it has room, in tensor memory (nine prompts 3 % quicker)
 //   softmax      a thread reads its row; the weights go back over S as FP16, with a factor of 2^6 that leaves small
 //                ones their bits (the sum of the weights takes it out)
 //   O += P V     weights from tensor memory, values feature-major
 // so a tile of the cache is unpacked once for 256 rows, and one tile's products run beside the other's softmax.
-// BF16 queries become FP16 numbers times a power of two of their row.  The running maximum moves when the weights of 64
-// positions add up to more than 2^8 of its own; sums are FP32.  A position that a row does not see is masked before the
-// maximum, and values are finite (append marks a NaN in the key), so nothing behind a row's own position reaches it.
+// BF16 queries become FP16 numbers times a power of two of their row.  The running maximum moves when a score exceeds it
+// by more than 2^8; sums are FP32.  A position that a row does not see is masked before the maximum, and values are
+// finite (append marks a NaN in the key), so nothing behind a row's own position reaches it.
 //
 // Work: tiles of rows, longest first; or, where there are too few, all tiles of positions as one sequence of which
 // every CTA takes an equal part, parts of a tile of rows joined by a second launch in their order.
 // All mbarrier waits are bounded.
 //
-// What bounds it: 512 tokens of 32 heads of 128 over 8 behind 16000 take 158 - 172 us, 0.8 - 0.87 PFLOP/s (the power
-// limit decides); without the softmax arithmetic it would be 125, without the products 149, without the exponentials
-// 141: issue of the softmax warps and the tensor pipe, nearly level.  Heads of 64 have half the products for the same
-// softmax: nine prompts of 4529 tokens in all take 120, of which the exponentials alone are 28 at 16 a clock and SM.
+// What bounds it: 512 tokens of 32 heads of 128 over 8 behind 16000 take 148 - 162 us, 0.84 - 0.92 PFLOP/s (the power
+// limit decides), 136 without the exponentials; before the scores were read twice, 158, it was 125 without any softmax
+// arithmetic and 149 without the products: the softmax warps, then the tensor pipe.  Heads of 64 have half the products for the same
+// softmax: nine prompts of 4529 tokens in all take 115, 99 without the exponentials, of which 28 are their full rate.
 #include <cmath>
 #include <type_traits>
 
@@ -43,7 +43,7 @@ constexpr int kThreads = 512;                        // warps: softmax of a tile
 constexpr int kUnpackThreads = 96;                   // of keys, and of values
 constexpr int kBlock = kTile * 128;                  // bytes of 64 columns of a tile: 128-byte rows
 constexpr int kStages = 2, kHalf = kTile / 2;
-constexpr float kLift = 6.f, kMost = 16384.f, kLog2e = 1.4426950408889634f;          // kMost: 2^8 times what kLift lifts
+constexpr float kLift = 6.f, kSlack = 8.f, kLog2e = 1.4426950408889634f;             // 2^(kLift + kSlack) fits FP16
 
 template <int DIM, int ROW_TILES>
 struct Prompt {
@@ -467,48 +467,26 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
                 ok = __all_sync(0xffffffffu, mbar_wait(bar(kSFull + u), parity, abortp));
                 if (!ok) break;
                 fence_after();
-                bool again = false;
-                uint32_t s[2][32];
-                tmem_ld32(at_s, s[0]);
-                tmem_ld32(at_s + 32, s[1]);
-                wait_ld();
-                if ((j + 1) * kHalf > least) {                              // some (row, position) is masked
-                    const int seen = sees - j * kHalf;
+                const int seen = sees - j * kHalf;
+                const bool masked = (j + 1) * kHalf > least;                // some (row, position)
+                float mx;
+                {
+                    uint32_t s[2][32];
+                    tmem_ld32(at_s, s[0]);
+                    tmem_ld32(at_s + 32, s[1]);
+                    wait_ld();
+                    if (masked) {
 #pragma unroll
-                    for (int k = 0; k < kHalf; k++)
-                        if (k >= seen) s[k / 32][k % 32] = 0xff800000u;
-                }
-                // With the maximum so far.  It is looked for only where the sum of the half's weights shows that one may exceed 2^kSlack, and for
-                // the first half; a second pass follows.
-                f32x2 sum[2];
-                uint32_t pw[32];
-#pragma unroll 1
-                for (bool first = j == 2 * w.j0;; first = false) {
-                    float total = INFINITY;
-                    if (!first) {
-                        const float ref = kLift - (m == -INFINITY ? 0.f : m);
-                        const f32x2 off = pair_f32(ref, ref);
-                        sum[0] = sum[1] = 0ull;
-#pragma unroll
-                        for (int k = 0; k < 32; k++) {
-                            const uint32_t(&v)[32] = s[k / 16];
-                            const float2 e = split_f32(fma_pairs(pair_f32(v[k % 16 * 2], v[k % 16 * 2 + 1]), scale, off));
-                            const float x = exp2_neg(e.x), y = exp2_neg(e.y);
-                            sum[k & 1] = add_pair(sum[k & 1], pair_f32(x, y));
-                            pw[k] = Pair2<half>::of(x, y);
-                        }
-                        total = sum_pair(add_pair(sum[0], sum[1]));
+                        for (int k = 0; k < kHalf; k++)
+                            if (k >= seen) s[k / 32][k % 32] = 0xff800000u;
                     }
-                    if (again || !__any_sync(0xffffffffu, !(total <= kMost))) {
-                        l += total;
-                        break;
-                    }
-                    again = true;
                     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int k = 0; k < 32; k++) top[k & 1] = max3(top[k & 1], __uint_as_float(s[k / 16][k % 16 * 2]), __uint_as_float(s[k / 16][k % 16 * 2 + 1]));
-                    const float mx = max3(top[0], top[0], top[1]) * scale2;
-                    const bool grows = !(total <= kMost) && mx > m;         // a row's result does not depend on the others' of its warp
+                    for (int k = 0; k < 32; k++) top[k / 16] = max3(top[k / 16], __uint_as_float(s[k / 16][k % 16 * 2]), __uint_as_float(s[k / 16][k % 16 * 2 + 1]));
+                    mx = max3(top[0], top[0], top[1]) * scale2;
+                }
+                const bool grows = !(mx <= m + kSlack);                     // a row's result does not depend on the others' of its warp
+                if (__any_sync(0xffffffffu, grows)) {
                     const float f = grows ? exp2_neg(m - mx) : 1.f;         // 0 where nothing was seen before
                     if (grows) {
                         m = mx;
@@ -531,8 +509,31 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
                         }
                     }
                 }
-                if (!ok) break;
-                tmem_st32(at_s, pw);
+                // The scores are read again, 32 at once: kept since the search for the maximum they take the registers that exponentials ahead
+                // of their use need (512 behind 16000 158 us, 148.5 read again, 16 at once 156).
+                const float ref = kLift - (m == -INFINITY ? 0.f : m);
+                const f32x2 off = pair_f32(ref, ref);
+                f32x2 sum[2] = {0ull, 0ull};
+#pragma unroll
+                for (int c = 0; c < kHalf; c += 32) {
+                    uint32_t s[32], pw[16];
+                    tmem_ld32(at_s + c, s);
+                    wait_ld();
+                    if (masked) {
+#pragma unroll
+                        for (int k = 0; k < 32; k++)
+                            if (c + k >= seen) s[k] = 0xff800000u;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const float2 e = split_f32(fma_pairs(pair_f32(s[2 * k], s[2 * k + 1]), scale, off));
+                        const float x = exp2_neg(e.x), y = exp2_neg(e.y);
+                        sum[k & 1] = add_pair(sum[k & 1], pair_f32(x, y));
+                        pw[k] = Pair2<half>::of(x, y);
+                    }
+                    tmem_st16(at_s + c / 2, pw);                            // over scores that were read
+                }
+                l += sum_pair(add_pair(sum[0], sum[1]));
                 wait_st();
                 fence_before();
                 mbar_arrive(bar(kPReady + u));
