@@ -194,7 +194,8 @@ int tllm_b200_cache4_attention(const tllm_b200_cache4* cache, int type, const in
     int st;
     if ((st = check_type(fn, type, false)) || (st = check_cache(fn, cache, &a.c)) || (st = check_seqs(fn, first, lens, tokens, a.c, &a.s)) ||
         (st = check_heads(fn, a.c, tokens, heads, max_new, max_len)) || (st = check_rows(fn, "q", q, type, tokens, heads, a.c.dim)) ||
-        (st = check_rows(fn, "out", out_rows, type, tokens, heads, a.c.dim)) || (st = check_apart(fn, "q", q, heads, out_rows, heads, type, a.c.batch ? tokens : 0, a.c.dim, false)))
+        (st = check_rows(fn, "out", out_rows, type, tokens, heads, a.c.dim)) ||
+        (st = check_apart(fn, "q", q, heads, out_rows, heads, type, a.c.batch ? tokens : 0, a.c.dim, false)))
         return st;
     if (!std::isfinite(scale)) return fail(TLLM_ERR_SHAPE, "cache4_attention: scale %g", scale);
     a.heads = heads;
