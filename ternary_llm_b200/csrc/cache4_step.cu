@@ -246,7 +246,7 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
         least = min(least, __shfl_xor_sync(0xffffffffu, least, 2));        // every row of the tile sees so many positions
 
         float m[NS], ref[NS], l[NS], lo[NS][GR], o[NC][GR][4][4];          // ref: m, 0 before the first position
-        float largest = 0.f, unit = 0.f;                                   // power of two above every scale of values so far, kLift / it
+        float largest = 0.f, unit = 0.f;                                   // power of two above the size of every scale of values so far, kLift / it
 #pragma unroll
         for (int n = 0; n < NS; n++) {
             m[n] = -INFINITY;
@@ -295,7 +295,7 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                         par[u][gr] = __half22float2(halves(kw[gr]));
                         vpar[h][u][gr] = __half22float2(halves(vw[gr]));
                         vpar[h][u][gr].y = fmaf(8.f, vpar[h][u][gr].x, vpar[h][u][gr].y);
-                        grows = grows || vpar[h][u][gr].x > largest;
+                        grows = grows || fabsf(vpar[h][u][gr].x) > largest;
                     }
                 }
 #pragma unroll
@@ -340,7 +340,7 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
 #pragma unroll
                     for (int u = 0; u < 2; u++)
 #pragma unroll
-                        for (int gr = 0; gr < GR; gr++) top = fmaxf(top, vpar[h][u][gr].x);
+                        for (int gr = 0; gr < GR; gr++) top = fmaxf(top, fabsf(vpar[h][u][gr].x));
                 top = warp_max(top);
                 if (top > largest) top = __int_as_float(((__float_as_int(top) >> 23) + 1) << 23);
                 const float shrink = top > largest ? largest / top : 1.f;
