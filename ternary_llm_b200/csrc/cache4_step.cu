@@ -6,10 +6,11 @@
 //            query is 16 bits of its largest entry in the group, as two signed bytes in neighbouring columns of the
 //            product (m16n8k32), whose sums are joined exactly.  Positions are the rows of the product.
 //   outputs  sum_p (w s) (c - 8) + sum_p w (l + 8 s)   codes are FP16 numbers after a mask and an addition or
-//            multiplication for two, w s is rounded to FP16 (11 bits of it, with a power of two that follows the largest
-//            scale seen, so that small scales do not run out of exponents) and meets the difference from the middle of
-//            the group's range; the second sum is FP32.  Channels are the rows of the product (m16n8k16), columns the
-//            query rows, or with up to four of them the four for the first and the four for the second group.
+//            multiplication for two, w s is rounded to FP16 (11 bits of it) and meets the difference from the middle of
+//            the group's range; the second sum is FP32.  w s is in units of its row and group that follow the largest w |s| of
+//            the positions that the row sees, so that a scale far above it without weight takes no bits: they are lost from
+//            2^-20 of it on, in steps of 2^-30 of it.  Channels are the rows of the product (m16n8k16), columns the query
+//            rows, or with up to four of them the four for the first and the four for the second group.
 // Weights come out of the first product by position and go into the second as pairs of positions: movmatrix, an 8 x 8
 // transposition in registers.  The running maximum moves when a score exceeds it by more than 2^8; sums are FP32.
 //
@@ -30,7 +31,7 @@ namespace tllm {
 namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr float kSlack = 8.f, kLift = 16.f;
+constexpr float kSlack = 8.f, kLift = 64.f, kMost = 32768.f;          // kMost: of a weight times a scale in units, inside FP16
 constexpr int kPad = 8;                                     // floats behind a row of a warp's outputs
 constexpr float kDigits = 32512.f;                          // largest query entry in the integer product: 127 * 256
 
@@ -85,6 +86,29 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v)
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+
+// The largest of the eight lanes that hold a row.
+__device__ __forceinline__ float row_max(float v)
+{
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+    return v;
+}
+
+// The same of one or two numbers that are not negative, by their upper 16 bits.
+template <int N>
+__device__ __forceinline__ void row_max_upper(float (&v)[N])
+{
+    uint32_t x = __byte_perm(__float_as_uint(v[0]), __float_as_uint(v[N - 1]), 0x7632);
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) x = __vmaxu2(x, __shfl_xor_sync(0xffffffffu, x, d));
+    v[0] = __uint_as_float(x << 16);
+    v[N - 1] = __uint_as_float(x & 0xffff0000u);
+}
+
+// The power of two that takes v to kLift .. 2 kLift, for v of 2^-100 .. 2^30, and kLift divided by it (0 for 0).
+__device__ __forceinline__ float unit_of(float v) { return __int_as_float(((260 - (__float_as_int(v) >> 23)) << 23)); }
+__device__ __forceinline__ float unit_back(float unit) { return unit > 0.f ? unit_of(unit) : 0.f; }
 
 // Rows of a product 0..7 as positions: lanes of a quad-strided read then fall on different banks, for keys (rows 0..3
 // and 4..7 at once) and for values (even ones and odd ones at once).
@@ -246,13 +270,13 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
         least = min(least, __shfl_xor_sync(0xffffffffu, least, 2));        // every row of the tile sees so many positions
 
         float m[NS], ref[NS], l[NS], lo[NS][GR], o[NC][GR][4][4];          // ref: m, 0 before the first position
-        float largest = 0.f, unit = 0.f;                                   // power of two above the size of every scale of values so far, kLift / it
+        float unit[NS][GR];                                                // what weights times scales of values are multiplied with, 0 before the first
 #pragma unroll
         for (int n = 0; n < NS; n++) {
             m[n] = -INFINITY;
             ref[n] = l[n] = 0.f;
 #pragma unroll
-            for (int gr = 0; gr < GR; gr++) lo[n][gr] = 0.f;
+            for (int gr = 0; gr < GR; gr++) lo[n][gr] = unit[n][gr] = 0.f;
         }
 #pragma unroll
         for (int n = 0; n < NC; n++)
@@ -275,7 +299,6 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
 
             // ---- scores ----
             float s[NS][2][2];                                             // set, half of the chunk, row g or g + 8 of the product
-            bool grows = false;
             float2 vpar[2][2][GR];                                         // (s, l + 8 s) of values
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -295,7 +318,6 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                         par[u][gr] = __half22float2(halves(kw[gr]));
                         vpar[h][u][gr] = __half22float2(halves(vw[gr]));
                         vpar[h][u][gr].y = fmaf(8.f, vpar[h][u][gr].x, vpar[h][u][gr].y);
-                        grows = grows || fabsf(vpar[h][u][gr].x) > largest;
                     }
                 }
 #pragma unroll
@@ -331,41 +353,55 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                         for (int u = 0; u < 2; u++)
                             if (p0 + 16 * h + 8 * u + place(g) >= sees[n]) s[n][h][u] = -INFINITY;
             }
+            // A row's maximum moves with its scores, its unit with its weights times scales; the largest of either says whether they may have to.
+            bool grows = false;
+            float scales[GR];
 #pragma unroll
-            for (int n = 0; n < NS; n++) grows = grows || fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][1][0], s[n][1][1])) > m[n] + kSlack;
+            for (int gr = 0; gr < GR; gr++) scales[gr] = fmaxf(fmaxf(fabsf(vpar[0][0][gr].x), fabsf(vpar[0][1][gr].x)), fmaxf(fabsf(vpar[1][0][gr].x), fabsf(vpar[1][1][gr].x)));
+#pragma unroll
+            for (int n = 0; n < NS; n++) {
+                const float v = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][1][0], s[n][1][1])), p = exp2_neg(v - ref[n]);
+                grows = grows || v > m[n] + kSlack;
+#pragma unroll
+                for (int gr = 0; gr < GR; gr++) grows = grows || p * unit[n][gr] * scales[gr] > kMost;
+            }
             if (__any_sync(0xffffffffu, grows)) {
-                float top = largest;
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++)
-#pragma unroll
-                        for (int gr = 0; gr < GR; gr++) top = fmaxf(top, fabsf(vpar[h][u][gr].x));
-                top = warp_max(top);
-                if (top > largest) top = __int_as_float(((__float_as_int(top) >> 23) + 1) << 23);
-                const float shrink = top > largest ? largest / top : 1.f;
-                largest = top;
-                unit = top > 0.f ? kLift / top : 0.f;
+                // each row by what it sees itself: its result does not depend on the others of the tile
 #pragma unroll
                 for (int n = 0; n < NS; n++) {
-                    float v = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][1][0], s[n][1][1]));
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                    const float f = v > m[n] ? exp2_neg(m[n] - v) : 1.f;
-                    m[n] = fmaxf(m[n], v);
-                    ref[n] = m[n] == -INFINITY ? 0.f : m[n];
+                    const float v = row_max(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][1][0], s[n][1][1])));
+                    const bool up = v > m[n] + kSlack;
+                    const float f = up ? exp2_neg(m[n] - v) : 1.f;
+                    if (up) m[n] = ref[n] = v;
                     l[n] *= f;
+                    float here[GR] = {};
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const float p = exp2_neg(s[n][h][u] - ref[n]);
+#pragma unroll
+                            for (int gr = 0; gr < GR; gr++) here[gr] = fmaxf(here[gr], p * fabsf(vpar[h][u][gr].x));
+                        }
+                    row_max_upper(here);
 #pragma unroll
                     for (int gr = 0; gr < GR; gr++) {
+                        const float most = here[gr];
+                        float by = f;
+                        if (up || most * unit[n][gr] > kMost) {
+                            const float back = unit_back(unit[n][gr]), now = unit_of(fmaxf(fmaxf(back * f, most), 0x1p-100f));
+                            by = f * (back * now * (1.f / kLift));
+                            unit[n][gr] = now;
+                        }
                         lo[n][gr] *= f;
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             if constexpr (ROWS == 4) {
-                                o[0][gr][k][gr] *= f * shrink;
-                                o[0][gr][k][2 + gr] *= f * shrink;
+                                o[0][gr][k][gr] *= by;
+                                o[0][gr][k][2 + gr] *= by;
                             } else {
-                                o[n >> 1][gr][k][n & 1] *= f * shrink;
-                                o[n >> 1][gr][k][2 + (n & 1)] *= f * shrink;
+                                o[n >> 1][gr][k][n & 1] *= by;
+                                o[n >> 1][gr][k][2 + (n & 1)] *= by;
                             }
                         }
                     }
@@ -378,25 +414,26 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
                 uint32_t pw[NC][GR][2];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    float p[NS], f[GR];
-#pragma unroll
-                    for (int gr = 0; gr < GR; gr++) f[gr] = vpar[h][u][gr].x * unit;
+                    float p[NS], ps[NS][GR];                               // weights; times the scales of values, in units
 #pragma unroll
                     for (int n = 0; n < NS; n++) {
                         p[n] = exp2_neg(s[n][h][u] - ref[n]);
                         l[n] += p[n];
 #pragma unroll
-                        for (int gr = 0; gr < GR; gr++) lo[n][gr] = fmaf(p[n], vpar[h][u][gr].y, lo[n][gr]);
+                        for (int gr = 0; gr < GR; gr++) {
+                            ps[n][gr] = p[n] * (vpar[h][u][gr].x * unit[n][gr]);
+                            lo[n][gr] = fmaf(p[n], vpar[h][u][gr].y, lo[n][gr]);
+                        }
                     }
                     if constexpr (ROWS == 4) {
-                        pw[0][0][u] = transposed(bits(__floats2half2_rn(p[0] * f[0], GR == 2 ? p[0] * f[GR - 1] : 0.f)));
+                        pw[0][0][u] = transposed(bits(__floats2half2_rn(ps[0][0], GR == 2 ? ps[0][GR - 1] : 0.f)));
 #pragma unroll
                         for (int gr = 1; gr < GR; gr++) pw[0][gr][u] = pw[0][0][u];
                     } else {
 #pragma unroll
                         for (int n = 0; n < NC; n++)
 #pragma unroll
-                            for (int gr = 0; gr < GR; gr++) pw[n][gr][u] = transposed(bits(__floats2half2_rn(p[2 * n] * f[gr], p[2 * n + 1] * f[gr])));
+                            for (int gr = 0; gr < GR; gr++) pw[n][gr][u] = transposed(bits(__floats2half2_rn(ps[2 * n][gr], ps[2 * n + 1][gr])));
                     }
                 }
 #pragma unroll
@@ -440,7 +477,7 @@ cache4_step_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> out,
 #pragma unroll
             for (int gr = 0; gr < GR; gr++) {
                 float* y = outs + warp * St::kOut + r * (DIM + kPad) + 64 * gr + 8 * g;
-                const float back = largest / kLift;
+                const float back = unit_back(unit[n][gr]) * (1.f / kLift);
                 const int nc = ROWS == 4 ? 0 : n >> 1, e = ROWS == 4 ? gr : n & 1;
 #pragma unroll
                 for (int k = 0; k < 4; k += 2)
