@@ -9,7 +9,8 @@ append, read back and attention for sequences of different lengths in one call.
 Activations are [tokens, heads, dim] (rows may lie apart, as parts of a wider tensor do); sequence b has the
 rows first[b] .. first[b + 1] - 1, at the last of its lens[b] positions; both are int32 CUDA tensors.  Checks
 of types, shapes and devices, then one call of the C ABI on torch's current stream; nothing here computes with
-torch operations.
+torch operations.  A cache and a table stand for the memory that they were made of: a call is refused once one of their
+tensors is at other memory, or its storage has another size.
 """
 from __future__ import annotations
 
@@ -65,11 +66,29 @@ def rotary_turns(frequencies):
 
 
 class _Fixed:
-    """What native calls keep the addresses of: set once."""
-    _bytes = None
+    """A C struct that begins with the addresses of tensors, set once.  The tensors are asked in each call whether they are still at that memory."""
+    _native = None
+
+    def _keep(self, struct, *tensors):
+        """Native calls take the struct as it is here; any device or layout that they cannot take goes through _desc, which says what is wrong."""
+        for t in tensors:
+            if t.numel() and (t.storage_offset() + t.numel()) * t.element_size() > t.untyped_storage().nbytes():
+                raise ValueError(f"a tensor of {tuple(t.shape)} whose storage holds {t.untyped_storage().nbytes()} bytes")
+        parts = (part for t in tensors for s in (t.untyped_storage(),) for part in (t, s, s.nbytes()))
+        device = tensors[0].get_device() if all(t.is_cuda and t.is_contiguous() and t.device == tensors[0].device for t in tensors) else -1
+        self._native = bytes(struct), device, *parts
+
+    def _same(self, struct, *names):
+        """The struct, which names the tensors' present addresses, where these are what the handle was made of."""
+        parts = self._native[2:]
+        for i, name in enumerate(names):
+            t, s, n = parts[3 * i:3 * i + 3]
+            if s.nbytes() != n or bytes(struct)[8 * i:8 * i + 8] != self._native[0][8 * i:8 * i + 8]:
+                raise ValueError(f"the memory of {name} is not what it was: make another {type(self).__name__}")
+        return struct
 
     def __setattr__(self, name, value):
-        if self._bytes is not None:
+        if self._native is not None:
             raise AttributeError(f"{type(self).__name__}.{name} cannot be changed: make another {type(self).__name__}")
         object.__setattr__(self, name, value)
 
@@ -90,8 +109,7 @@ class RotaryTable(_Fixed):
         self.amplitude = own if amplitude is None else float(amplitude)
         turns = torch.frombuffer(_turns(f, rot_dim // 2), dtype=torch.int64, count=rot_dim // 2)
         self.turns = turns.clone() if device is not None and torch.device(device).type == "cpu" else turns.to("cuda" if device is None else device)
-        self._device = self.turns.get_device()
-        self._bytes = bytes(_lib.RotaryTableDesc(self.turns.data_ptr(), rot_dim, int(half), self.amplitude))
+        self._keep(_lib.RotaryTableDesc(self.turns.data_ptr(), rot_dim, int(half), self.amplitude), self.turns)
 
     def __reduce__(self):
         return RotaryTable, (self.rot_dim, 0.0, self.half, None, self.frequencies, self.amplitude, str(self.turns.device))
@@ -101,7 +119,7 @@ class RotaryTable(_Fixed):
         return list(self._f)[:self.rot_dim // 2]
 
     def _desc(self):
-        return _lib.RotaryTableDesc(_chk(self.turns, torch.int64, "turns", self.rot_dim // 2), self.rot_dim, int(self.half), self.amplitude)
+        return self._same(_lib.RotaryTableDesc(_chk(self.turns, torch.int64, "turns", self.rot_dim // 2), self.rot_dim, int(self.half), self.amplitude), "turns")
 
 
 class Cache4(_Fixed):
@@ -119,12 +137,9 @@ class Cache4(_Fixed):
             if tuple(t.shape) != tuple(shape):
                 raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
-        # for the native calls; any other device or layout goes through _desc, which says what is wrong
         all4 = (k_codes, k_params, v_codes, v_params)
-        fit = k_codes.is_cuda and all(t.is_contiguous() and t.device == k_codes.device for t in all4) and \
-            k_codes.dtype == v_codes.dtype == torch.uint8 and k_params.dtype == v_params.dtype == torch.float16
-        self._device = k_codes.get_device() if fit else -1
-        self._bytes = bytes(_lib.Cache4Desc(*(t.data_ptr() for t in all4), self.batch, self.kv_heads, self.rows, self.dim)) if fit else b""
+        types = tuple(t.dtype for t in all4) == (torch.uint8, torch.float16) * 2
+        self._keep(_lib.Cache4Desc(*(t.data_ptr() if types else None for t in all4), self.batch, self.kv_heads, self.rows, self.dim), *all4)
 
     def __reduce__(self):
         return Cache4, (self.k_codes, self.k_params, self.v_codes, self.v_params)
@@ -137,9 +152,9 @@ class Cache4(_Fixed):
                      for last, t in (((dim // 2,), torch.uint8), ((dim // GROUP, 2), torch.float16)) * 2))
 
     def _desc(self):
-        return _lib.Cache4Desc(_chk(self.k_codes, torch.uint8, "k_codes"), _chk(self.k_params, torch.float16, "k_params"),
-                               _chk(self.v_codes, torch.uint8, "v_codes"), _chk(self.v_params, torch.float16, "v_params"),
-                               self.batch, self.kv_heads, self.rows, self.dim)
+        return self._same(_lib.Cache4Desc(_chk(self.k_codes, torch.uint8, "k_codes"), _chk(self.k_params, torch.float16, "k_params"),
+                                          _chk(self.v_codes, torch.uint8, "v_codes"), _chk(self.v_params, torch.float16, "v_params"),
+                                          self.batch, self.kv_heads, self.rows, self.dim), "k_codes", "k_params", "v_codes", "v_params")
 
 
 def _rows(t, dtype, name: str, tokens: int, heads: int, dim: int):
@@ -174,7 +189,7 @@ def _ref(d):
 def rotary(q, k, positions, table: RotaryTable, q_out=None, k_out=None, inverse: bool = False) -> None:
     """Turns q [tokens, heads, dim] and k [tokens, kv_heads, dim] (or None) by positions int32 [tokens], in place where no
     output is given; inverse turns back (the gradient).  FP16, BF16 or FP32."""
-    st = _lib.host().rotary(table._bytes, table._device, q, k, positions, q_out, k_out, inverse)
+    st = _lib.host().rotary(table._native, q, k, positions, q_out, k_out, inverse)
     if st is not None:
         return _lib.check(st)
     kind = _type(q, "q", tuple(TYPES))
@@ -191,8 +206,7 @@ def rotary(q, k, positions, table: RotaryTable, q_out=None, k_out=None, inverse:
 
 def append(cache: Cache4, q, k, v, first, lens, table: RotaryTable | None = None, q_out=None) -> None:
     """Turns q (or None) into q_out (default: in place) and k, and writes k and v to the cache.  FP16 or BF16."""
-    st = _lib.host().cache4_append(cache._bytes, cache._device, None if table is None else table._bytes, 0 if table is None else table._device, q, k, v,
-                                   first, lens, q_out)
+    st = _lib.host().cache4_append(cache._native, None if table is None else table._native, q, k, v, first, lens, q_out)
     if st is not None:
         return _lib.check(st)
     kind = _type(k, "k", (torch.float16, torch.bfloat16))
@@ -211,7 +225,7 @@ def append(cache: Cache4, q, k, v, first, lens, table: RotaryTable | None = None
 def read(cache: Cache4, k, v, first, lens) -> None:
     """Writes the keys and values at the rows' positions, as the cache holds them, to k and v [tokens, kv_heads, dim] (one of
     them may be None).  FP16, BF16 or FP32."""
-    st = _lib.host().cache4_read(cache._bytes, cache._device, k, v, first, lens)
+    st = _lib.host().cache4_read(cache._native, k, v, first, lens)
     if st is not None:
         return _lib.check(st)
     some = v if k is None else k
@@ -230,7 +244,7 @@ def attention(cache: Cache4, q, out, first, lens, scale: float | None = None, ma
     sequence holds more positions (0: the cache's rows); workspaces are as large as that needs.  FP16 or BF16."""
     if scale is None:
         scale = cache.dim ** -0.5
-    st = _lib.host().cache4_attention(cache._bytes, cache._device, q, out, first, lens, scale, max_new, max_len)
+    st = _lib.host().cache4_attention(cache._native, q, out, first, lens, scale, max_new, max_len)
     if st is not None:
         return _lib.check(st)
     kind, d = _type(q, "q", (torch.float16, torch.bfloat16)), cache._desc()

@@ -5,7 +5,8 @@
  * the conversion of arguments, in front of a kernel of 3.2 us.  The functions here ask the tensors the same
  * questions and call the library, 4.1 us with the launch; where an answer is not the expected one, or an argument is not a plain
  * int or float, they return None and do nothing, and the caller goes through the checks in Python, which
- * say what is wrong.  Nothing is kept from one call for the next.
+ * say what is wrong.  Nothing is kept from one call for the next; the structs of a cache and a rotary table are made with
+ * them, and each call asks whether their memory is still there.
  *
  * The library's functions are handed over as addresses, so that whichever build of it is loaded is used. */
 #define PY_SSIZE_T_CLEAN
@@ -132,7 +133,8 @@ static PyObject* gemm_packed(PyObject* self, PyObject* const* a, Py_ssize_t n)
     return PyLong_FromLong(status);
 }
 
-/* ---- 4-bit cache: handles are the bytes of their C structs, made once by the Python objects that own the memory ---- */
+/* ---- 4-bit cache: handles are C structs made once by the Python objects that own the memory, and its tensors, which are asked each time whether they
+ * are still there ---- */
 static int (*f_rotary)(int, const tllm_b200_rotary_table*, const int*, int, const tllm_b200_heads*, const tllm_b200_heads*, int, const tllm_b200_heads*,
                        const tllm_b200_heads*, int, int, int, void*);
 static int (*f_append)(const tllm_b200_cache4*, int, const tllm_b200_rotary_table*, const int*, const int*, int, const tllm_b200_heads*,
@@ -142,7 +144,7 @@ static int (*f_attention)(const tllm_b200_cache4*, int, const int*, const int*, 
                           void*, size_t, void*);
 static int (*f_workspace)(const tllm_b200_cache4*, int, int, int, int, size_t*);
 static PyObject *d_types[3], *d_int32;                          /* FP16, BF16, FP32 as the C ABI numbers them */
-static PyObject *s_shape, *s_stride, *s_new_empty;
+static PyObject *s_shape, *s_stride, *s_new_empty, *s_nbytes;
 
 /* Three numbers of a tuple; consumes the reference. */
 static int triple(PyObject* o, long long* v)
@@ -183,12 +185,27 @@ static int rows3(PyObject* t, long long device, int* type, long long* shape, tll
     return 1;
 }
 
-/* The C struct that `o`, a bytes object made on `device`, holds. */
-static const void* handle(PyObject* o, PyObject* device, long long current, size_t size)
+/* 1: tensor and storage are still the memory that a handle was made of, `bytes` of storage and the tensor at `p` in it.  The handle holds the
+ * storage, so that its memory can only go by a change of its size. */
+static int same(PyObject* t, PyObject* storage, PyObject* bytes, const void* p)
 {
-    if (!PyBytes_CheckExact(o) || (size_t)PyBytes_GET_SIZE(o) != size || !PyLong_CheckExact(device) || PyLong_AsLong(device) != current) return NULL;
-    return PyBytes_AS_STRING(o);
+    return p && number(method(t, s_data_ptr)) == (long long)p && number(method(storage, s_nbytes)) == PyLong_AsLongLong(bytes);
 }
+
+/* The C struct that `o`, (struct, its device, then a tensor, its storage and the storage's bytes for each address that the struct begins with), holds,
+ * where they are the memory they were. */
+static const void* handle(PyObject* o, long long current, size_t size, int addresses)
+{
+    if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 2 + 3 * addresses) return NULL;
+    PyObject *b = PyTuple_GET_ITEM(o, 0), *device = PyTuple_GET_ITEM(o, 1);
+    if (!PyBytes_CheckExact(b) || (size_t)PyBytes_GET_SIZE(b) != size || !PyLong_CheckExact(device) || PyLong_AsLongLong(device) != current) return NULL;
+    void* const* p = (void* const*)PyBytes_AS_STRING(b);
+    for (int i = 0; i < addresses; i++)
+        if (!same(PyTuple_GET_ITEM(o, 2 + 3 * i), PyTuple_GET_ITEM(o, 3 + 3 * i), PyTuple_GET_ITEM(o, 4 + 3 * i), p[i])) return NULL;
+    return p;
+}
+static const tllm_b200_cache4* cache_of(PyObject* o, long long device) { return handle(o, device, sizeof(tllm_b200_cache4), 4); }
+static const tllm_b200_rotary_table* table_of(PyObject* o, long long device) { return handle(o, device, sizeof(tllm_b200_rotary_table), 1); }
 
 /* int32 tensors of batch + 1 and batch entries */
 static int sequences(const tllm_b200_cache4* c, PyObject* first, PyObject* lens, long long dev, void** f, void** n)
@@ -206,7 +223,7 @@ static int not_negative(PyObject* o)
     return over || v < 0 || v > INT_MAX ? -1 : (int)v;
 }
 
-/* (table, its device, q, k or None, positions, q_out or None, k_out or None, inverse) */
+/* (table, q, k or None, positions, q_out or None, k_out or None, inverse) */
 static PyObject* rotary(PyObject* self, PyObject* const* a, Py_ssize_t n)
 {
     long long dev, q3[3] = {-1, -1, -1}, k3[3];
@@ -214,24 +231,22 @@ static PyObject* rotary(PyObject* self, PyObject* const* a, Py_ssize_t n)
     int type = -1;
     tllm_b200_heads q, qo, k, ko;
     const tllm_b200_rotary_table* t;
-    if (n != 8 || !f_rotary || !where(&dev, &stream) || !(t = handle(a[0], a[1], dev, sizeof *t)) || !rows3(a[2], dev, &type, q3, &q) ||
-        !PyBool_Check(a[7]))
-        Py_RETURN_NONE;
-    const int keys = a[3] != Py_None;
+    if (n != 7 || !f_rotary || !where(&dev, &stream) || !(t = table_of(a[0], dev)) || !rows3(a[1], dev, &type, q3, &q) || !PyBool_Check(a[6])) Py_RETURN_NONE;
+    const int keys = a[2] != Py_None;
     k3[0] = q3[0], k3[1] = -1, k3[2] = q3[2];
-    if (!rows3(a[5] == Py_None ? a[2] : a[5], dev, &type, q3, &qo) || (!keys && a[6] != Py_None) ||
-        (keys && (!rows3(a[3], dev, &type, k3, &k) || !rows3(a[6] == Py_None ? a[3] : a[6], dev, &type, k3, &ko))) ||
-        !tensor(a[4], d_int32, dev, q3[0], &positions))
+    if (!rows3(a[4] == Py_None ? a[1] : a[4], dev, &type, q3, &qo) || (!keys && a[5] != Py_None) ||
+        (keys && (!rows3(a[2], dev, &type, k3, &k) || !rows3(a[5] == Py_None ? a[2] : a[5], dev, &type, k3, &ko))) ||
+        !tensor(a[3], d_int32, dev, q3[0], &positions))
         Py_RETURN_NONE;
     int status;
     Py_BEGIN_ALLOW_THREADS
     status = f_rotary(type, t, positions, (int)q3[0], &q, &qo, (int)q3[1], keys ? &k : NULL, keys ? &ko : NULL, keys ? (int)k3[1] : 0, (int)q3[2],
-                      a[7] == Py_True, stream);
+                      a[6] == Py_True, stream);
     Py_END_ALLOW_THREADS
     return PyLong_FromLong(status);
 }
 
-/* (cache, its device, table or None, its device, q or None, k, v, first, lens, q_out or None) */
+/* (cache, table or None, q or None, k, v, first, lens, q_out or None) */
 static PyObject* cache4_append(PyObject* self, PyObject* const* a, Py_ssize_t n)
 {
     long long dev, q3[3], k3[3] = {-1, -1, -1};
@@ -240,15 +255,13 @@ static PyObject* cache4_append(PyObject* self, PyObject* const* a, Py_ssize_t n)
     tllm_b200_heads q, qo, k, v;
     const tllm_b200_cache4* c;
     const tllm_b200_rotary_table* t = NULL;
-    if (n != 10 || !f_append || !where(&dev, &stream) || !(c = handle(a[0], a[1], dev, sizeof *c)) ||
-        (a[2] != Py_None && !(t = handle(a[2], a[3], dev, sizeof *t))))
-        Py_RETURN_NONE;
+    if (n != 8 || !f_append || !where(&dev, &stream) || !(c = cache_of(a[0], dev)) || (a[1] != Py_None && !(t = table_of(a[1], dev)))) Py_RETURN_NONE;
     k3[1] = c->kv_heads, k3[2] = c->dim;
-    const int queries = a[4] != Py_None;
-    if (!rows3(a[5], dev, &type, k3, &k) || type == TLLM_FP32 || !rows3(a[6], dev, &type, k3, &v) || !sequences(c, a[7], a[8], dev, &first, &lens))
+    const int queries = a[2] != Py_None;
+    if (!rows3(a[3], dev, &type, k3, &k) || type == TLLM_FP32 || !rows3(a[4], dev, &type, k3, &v) || !sequences(c, a[5], a[6], dev, &first, &lens))
         Py_RETURN_NONE;
     q3[0] = k3[0], q3[1] = -1, q3[2] = c->dim;
-    if ((!queries && a[9] != Py_None) || (queries && (!rows3(a[4], dev, &type, q3, &q) || !rows3(a[9] == Py_None ? a[4] : a[9], dev, &type, q3, &qo))))
+    if ((!queries && a[7] != Py_None) || (queries && (!rows3(a[2], dev, &type, q3, &q) || !rows3(a[7] == Py_None ? a[2] : a[7], dev, &type, q3, &qo))))
         Py_RETURN_NONE;
     int status;
     Py_BEGIN_ALLOW_THREADS
@@ -257,7 +270,7 @@ static PyObject* cache4_append(PyObject* self, PyObject* const* a, Py_ssize_t n)
     return PyLong_FromLong(status);
 }
 
-/* (cache, its device, k or None, v or None, first, lens) */
+/* (cache, k or None, v or None, first, lens) */
 static PyObject* cache4_read(PyObject* self, PyObject* const* a, Py_ssize_t n)
 {
     long long dev, k3[3] = {-1, -1, -1};
@@ -265,19 +278,19 @@ static PyObject* cache4_read(PyObject* self, PyObject* const* a, Py_ssize_t n)
     int type = -1;
     tllm_b200_heads k, v;
     const tllm_b200_cache4* c;
-    if (n != 6 || !f_read || !where(&dev, &stream) || !(c = handle(a[0], a[1], dev, sizeof *c)) || (a[2] == Py_None && a[3] == Py_None)) Py_RETURN_NONE;
+    if (n != 5 || !f_read || !where(&dev, &stream) || !(c = cache_of(a[0], dev)) || (a[1] == Py_None && a[2] == Py_None)) Py_RETURN_NONE;
     k3[1] = c->kv_heads, k3[2] = c->dim;
-    if ((a[2] != Py_None && !rows3(a[2], dev, &type, k3, &k)) || (a[3] != Py_None && !rows3(a[3], dev, &type, k3, &v)) ||
-        !sequences(c, a[4], a[5], dev, &first, &lens))
+    if ((a[1] != Py_None && !rows3(a[1], dev, &type, k3, &k)) || (a[2] != Py_None && !rows3(a[2], dev, &type, k3, &v)) ||
+        !sequences(c, a[3], a[4], dev, &first, &lens))
         Py_RETURN_NONE;
     int status;
     Py_BEGIN_ALLOW_THREADS
-    status = f_read(c, type, first, lens, (int)k3[0], a[2] != Py_None ? &k : NULL, a[3] != Py_None ? &v : NULL, stream);
+    status = f_read(c, type, first, lens, (int)k3[0], a[1] != Py_None ? &k : NULL, a[2] != Py_None ? &v : NULL, stream);
     Py_END_ALLOW_THREADS
     return PyLong_FromLong(status);
 }
 
-/* (cache, its device, q, out, first, lens, scale, max_new, max_len); the workspace is a tensor of the call's own */
+/* (cache, q, out, first, lens, scale, max_new, max_len); the workspace is a tensor of the call's own */
 static PyObject* cache4_attention(PyObject* self, PyObject* const* a, Py_ssize_t n)
 {
     long long dev, q3[3] = {-1, -1, -1};
@@ -286,18 +299,18 @@ static PyObject* cache4_attention(PyObject* self, PyObject* const* a, Py_ssize_t
     size_t need = 0;
     tllm_b200_heads q, out;
     const tllm_b200_cache4* c;
-    if (n != 9 || !f_attention || !where(&dev, &stream) || !(c = handle(a[0], a[1], dev, sizeof *c)) || !PyFloat_CheckExact(a[6])) Py_RETURN_NONE;
-    const int max_new = not_negative(a[7]), max_len = not_negative(a[8]);
+    if (n != 8 || !f_attention || !where(&dev, &stream) || !(c = cache_of(a[0], dev)) || !PyFloat_CheckExact(a[5])) Py_RETURN_NONE;
+    const int max_new = not_negative(a[6]), max_len = not_negative(a[7]);
     q3[2] = c->dim;
-    if (max_new < 0 || max_len < 0 || !rows3(a[2], dev, &type, q3, &q) || type == TLLM_FP32 || !rows3(a[3], dev, &type, q3, &out) ||
-        !sequences(c, a[4], a[5], dev, &first, &lens))
+    if (max_new < 0 || max_len < 0 || !rows3(a[1], dev, &type, q3, &q) || type == TLLM_FP32 || !rows3(a[2], dev, &type, q3, &out) ||
+        !sequences(c, a[3], a[4], dev, &first, &lens))
         Py_RETURN_NONE;
     int status = f_workspace(c, (int)q3[0], (int)q3[1], max_new, max_len, &need);
     if (status) return PyLong_FromLong(status);
     PyObject* memory = NULL;
     if (need) {
         PyObject* size = PyLong_FromSize_t((need + 1) / 2);               /* q's type has two bytes */
-        memory = size ? PyObject_CallMethodOneArg(a[2], s_new_empty, size) : NULL;
+        memory = size ? PyObject_CallMethodOneArg(a[1], s_new_empty, size) : NULL;
         Py_XDECREF(size);
         if (!memory) return NULL;                                         /* out of memory, as torch says it */
         const long long p = number(method(memory, s_data_ptr));
@@ -307,7 +320,7 @@ static PyObject* cache4_attention(PyObject* self, PyObject* const* a, Py_ssize_t
         }
         ws = (void*)p;
     }
-    const float scale = (float)PyFloat_AS_DOUBLE(a[6]);
+    const float scale = (float)PyFloat_AS_DOUBLE(a[5]);
     Py_BEGIN_ALLOW_THREADS
     status = f_attention(c, type, first, lens, (int)q3[0], &q, &out, (int)q3[1], scale, max_new, max_len, ws, need, stream);
     Py_END_ALLOW_THREADS
@@ -375,7 +388,8 @@ PyMODINIT_FUNC PyInit__hostcall(void)
     s_shape = PyUnicode_InternFromString("shape");
     s_stride = PyUnicode_InternFromString("stride");
     s_new_empty = PyUnicode_InternFromString("new_empty");
-    if (!s_shape || !s_stride || !s_new_empty) return NULL;
+    s_nbytes = PyUnicode_InternFromString("nbytes");
+    if (!s_shape || !s_stride || !s_new_empty || !s_nbytes) return NULL;
     if (!s_is_cuda || !s_dtype || !s_is_contiguous || !s_get_device || !s_numel || !s_data_ptr) return NULL;
     return PyModule_Create(&module);
 }
