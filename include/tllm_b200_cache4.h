@@ -18,7 +18,7 @@
  * nothing is written for it, and its attention is 0.  first that does not rise or leaves 0..tokens, or
  * lens outside 0..rows, is cut to those limits and raises TLLM_ERR_SHAPE at the next
  * tllm_b200_check_device_errors; nothing outside the tensors is read or written.  (Where first falls,
- * attention may leave rows out.)
+ * attention writes nothing, and a row belongs to the first sequence that ends behind it for the others.)
  *
  * Activations: consecutive heads of a row lie behind one another, rows are ld elements apart, on 16-byte
  * boundaries.  All calls may be captured into graphs (once the library has been used on the device) and keep

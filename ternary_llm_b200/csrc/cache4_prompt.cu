@@ -219,7 +219,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) uint64_t bars[kBars];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, falls;
     __shared__ typename W::Base::Start start;
     __shared__ float row_scale[kRows];
     pdl_launch_dependents();
@@ -227,7 +227,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
     uint8_t *qs = smem, *ks = qs + ROW_TILES * P::kOperand, *vs = ks + kStages * P::kOperand, *raw = vs + kStages * P::kOperand;
     const uint32_t bar0 = smem_u32(bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
-    volatile int* abortp = &abort_flag;
+    volatile int *abortp = &abort_flag, *fallsp = &falls;
     int never = 0;
 
     if (tid == 0) {
@@ -236,7 +236,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
             mbar_init(bar(i), pair == kQFull || (i >= kPReady && i < kLast) ? kTile : pair == kKFull || pair == kVFull ? kUnpackThreads :
                               pair == kKEmpty || pair == kVEmpty ? ROW_TILES : 1);
         }
-        abort_flag = 0;
+        abort_flag = falls = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
     }
@@ -390,8 +390,16 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
     } else if (warp < 4 * ROW_TILES) {
         // ---------------- softmax: a row a thread ----------------
         const int i = warp >> 2, row = tid & (kTile - 1);
+        // Sequences of a call whose `first` falls may share rows: nothing is written then, as Work::find has it for work that is cut.  The 128 threads
+        // share the comparisons; each reads the others' answer behind kSFull, which comes behind their kQFull.
+        const bool mine = whole && row < a.s.batch;
+        const int from = mine ? a.s.first[row] : 0, upto = mine ? a.s.first[row + 1] : 0;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, row_s = tmem + i * kTile + lanes, row_o = tmem + ROW_TILES * kTile + i * DIM + lanes;
         W w(a, whole, start);
+        if (upto < from) *fallsp = 1;
+        if (whole)
+            for (int k = row + kTile; k < a.s.batch; k += kTile)
+                if (a.s.first[k + 1] < a.s.first[k]) *fallsp = 1;
         const bool wide = ((reinterpret_cast<uintptr_t>(out.p) | (uintptr_t)out.ld * sizeof(T)) & 31) == 0;     // outputs on whole sectors
         uint32_t rounds = 0;
         bool ok = true;
@@ -553,12 +561,13 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
                 rec[kRows + at] = l;
             }
             const float f = sees > 0 ? 1.f / l : 0.f;
+            const bool stores = there && !*fallsp;
 #pragma unroll 1
             for (int c = 0; c < DIM; c += 32) {
                 uint32_t o[32];
                 tmem_ld32(row_o + c, o);
                 wait_ld();
-                if (there && complete) {
+                if (stores && complete) {
                     uint32_t p[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++)
@@ -570,7 +579,7 @@ cache4_prompt_kernel(const Cache4Call a, const Rows<const T> q, const Rows<T> ou
 #pragma unroll
                         for (int e = 0; e < 4; e++) reinterpret_cast<uint4*>(y + c)[e] = make_uint4(p[4 * e], p[4 * e + 1], p[4 * e + 2], p[4 * e + 3]);
                     }
-                } else if (there) {
+                } else if (stores) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) store32(rec + 2 * kRows + at * DIM + c + e, o + e);
                 }

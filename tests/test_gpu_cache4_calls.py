@@ -1,0 +1,33 @@
+"""Calls of the 4-bit cache at the edges of what they are told: sequences that share rows, hints, parts of the work."""
+import numpy as np
+import pytest
+import torch
+
+import ternary_llm_b200 as tl
+from tests.test_gpu_cache4 import TYPES, check_attention, ints, layout, new_cache, random_cache
+from ternary_llm_b200 import cache4_ops as ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("first,lens,rows,heads,kv_heads,dim", [
+    ((0, 300, 200, 600), (300, 0, 400), 600, 8, 2, 64),            # whole tiles of 128 rows
+    ((0, 1200, 900, 2000), (1200, 0, 1100), 1200, 32, 8, 64),      # of 256
+    ((0, 300, 200, 600), (6000, 0, 6000), 6000, 8, 2, 128),        # cut
+    ((0, 1200, 900, 1800), (9000, 0, 9000), 9000, 32, 8, 128),
+    ((0, 2, 1, 4), (300, 0, 300), 300, 8, 2, 64),                  # few rows, in one CTA and cut
+    ((0, 2, 1, 4), (5000, 0, 5000), 5000, 8, 2, 64),
+    (tuple(range(700)) + (600, 710), (40,) * 701, 40, 4, 4, 64)])
+def test_sequences_that_share_rows(first, lens, rows, heads, kv_heads, dim):
+    """Attention writes nothing and says so."""
+    c = new_cache(len(lens), kv_heads, rows, dim)
+    for p in (c.k_params, c.v_params):
+        p.fill_(0.5)
+    q = torch.randn(first[-1], heads, dim, device="cuda").half()
+    new = max(max(b - a, 1) for a, b in zip(first, first[1:]))
+    for most in (new, 0, first[-1]):
+        out = torch.full_like(q, 7.0)
+        ops.attention(c, q, out, ints(*first), ints(*lens), max_new=most)
+        with pytest.raises(tl.TllmError, match="outside its tensors"):
+            tl.check_device_errors()
+        assert (out == 7).all()
