@@ -95,10 +95,11 @@ int tllm_b200_cache4_read(const tllm_b200_cache4* cache, int type, const int* fi
                           const tllm_b200_heads* v, void* stream);
 
 /* out = softmax(scale q . k) v over the positions up to the row's own, heads / kv_heads query heads to a
- * key/value head.  FP16 or BF16.  max_new: about the most rows of a sequence (0: not known), which chooses the
- * way of the work, not the result's meaning.  max_len: no sequence holds more positions (0: the cache's rows);
- * lens above it is cut and raises TLLM_ERR_SHAPE as lens above rows does.  workspace: device memory of
- * tllm_b200_cache4_workspace bytes on a 128-byte boundary, for this call alone. */
+ * key/value head.  FP16 or BF16.  max_new: about the most rows of a sequence (0: not known, then as many as
+ * they have on the average), which chooses the way of the work, not the result's meaning.  max_len: no sequence
+ * holds more positions (0: the cache's rows); lens above it is cut and raises TLLM_ERR_SHAPE as lens above rows
+ * does.  workspace: device memory of tllm_b200_cache4_workspace bytes on a 128-byte boundary, for this call
+ * alone. */
 int tllm_b200_cache4_attention(const tllm_b200_cache4* cache, int type, const int* first, const int* lens, int tokens,
                                const tllm_b200_heads* q, const tllm_b200_heads* out, int heads, float scale, int max_new, int max_len,
                                void* workspace, size_t workspace_bytes, void* stream);

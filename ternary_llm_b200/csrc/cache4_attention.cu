@@ -10,7 +10,7 @@ namespace tllm {
 // 300 9.3 / 14.3, behind 6000 49 / 34, 14 of 9 (336) behind 300 22 / 14, behind 2500 60 / 47.
 static bool takes_step(const Cache4& c, int tokens, int heads, int max_new, int max_len)
 {
-    const long long rows = (long long)(max_new > 0 && max_new < tokens ? max_new : tokens) * (heads / c.kv_heads);
+    const long long rows = (long long)new_rows(c, tokens, max_new) * (heads / c.kv_heads);
     const long long tiles = (rows + 15) / 16 * c.batch * c.kv_heads, len = max_len > 0 && max_len < c.rows ? max_len : c.rows;
     return rows <= 32 || (tiles <= 148 && (len <= kStepWhole / c.dim || tiles * len <= 40000000 / c.dim));
 }

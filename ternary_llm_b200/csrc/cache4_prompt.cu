@@ -625,6 +625,14 @@ PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int 
         const double by_tokens = (double)tokens * per / rows + c.batch, by_most = (double)c.batch * (((long long)most * per + rows - 1) / rows);
         return (by_tokens < by_most ? by_tokens : by_most) * c.kv_heads;
     };
+    // Whole tiles take CTAs for as many in every sequence as one may have, and 0.02 us a CTA that finds none: us, 32 heads of 128 over 8, whole / cut,
+    // 2000 tokens beside 3 single ones (740 such CTAs) 68 / 78, 15 (3700) 117 / 90, nine prompts of unknown length (3800) 137 / 117, 4000 beside 63 (31000) 630 / 256.
+    const long long pairs = (long long)c.batch * c.kv_heads;
+    const auto grid_of = [&](int rows) {
+        const long long grid = ((long long)most * per + rows - 1) / rows * pairs;
+        return grid < (1 << 20) ? grid : (1 << 20) / pairs * pairs;
+    };
+    const auto idle = [&](int rows) { return fmax(grid_of(rows) - ((double)tokens * per / rows + c.batch) * c.kv_heads, 0.0); };
     if (tiles_of(128) <= 148) {
         // An SM for each tile of 128 rows: the quickest of these tiles whole, cut, and tiles of 256 rows cut, as they measure, us: 8 + 1.9 for each
         // tile of positions, or 19 + 1.85 for each that a CTA takes, or 27 + 2.35; sequences of a batch differ, so that cut ones have fewer.
@@ -632,7 +640,7 @@ PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int 
         // 61; 500 behind 1200 36.4 / 48.2 / 42.0, behind 6000 111 / 117 / 85.  Tiles of 256 whole take 22.0, 60.9, 297, 42.8 and 131.
         const double few = c.batch > 1 ? 0.85 : 1;
         const auto cut = [&](int rows) { return fmax(tiles_of(rows) * (few * mean + Work<128, kTile>::kFixed) / 148, (double)Work<128, kTile>::kLeast); };
-        const double whole = 8 + 1.9 * longest, halves = 19 + 1.85 * cut(128), full = 27 + 2.35 * cut(256);
+        const double whole = 8 + 1.9 * longest + idle(128) / 75, halves = 19 + 1.85 * cut(128), full = 27 + 2.35 * cut(256);
         p.rows = full < fmin(whole, halves) ? 256 : 128;
         p.whole = whole <= fmin(halves, full);
     } else {
@@ -641,11 +649,9 @@ PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int 
         // 1500 39 whole, 57 cut, 2000 52 / 74; of 64, four prompts of 700 38 / 51.
         const double rows = (double)tokens * per / 256 > (double)c.batch ? (double)tokens * per / 256 : (double)c.batch;
         p.rows = 256;
-        p.whole = longest - rows * c.kv_heads * mean / 148 <= 7;
+        p.whole = longest - rows * c.kv_heads * mean / 148 <= 7 && idle(256) <= 1500;
     }
-    const long long tiles = ((long long)most * per + p.rows - 1) / p.rows, pairs = (long long)c.batch * c.kv_heads;
-    const long long grid = tiles * pairs < (1 << 20) ? tiles * pairs : (1 << 20) / pairs * pairs;
-    p.ctas = p.whole ? (int)(grid < pairs ? pairs : grid) : 148;
+    p.ctas = p.whole ? (int)fmax(grid_of(p.rows), pairs) : 148;
     p.bytes = p.whole ? 0 : join_bytes(c.dim, p.rows, p.ctas);
     return p;
 }

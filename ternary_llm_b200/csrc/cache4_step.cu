@@ -549,8 +549,7 @@ int launch_rows(const Cache4Call& a, Rows<const T> q, Rows<T> out, const StepPla
 StepPlan step_plan(const Cache4& c, int tokens, int heads, int max_new, int max_len)
 {
     StepPlan p;
-    const int per = heads / c.kv_heads, most = max_new > 0 && max_new < tokens ? max_new : (tokens + c.batch - 1) / c.batch;
-    const long long rows = (long long)most * per;
+    const long long rows = (long long)new_rows(c, tokens, max_new) * (heads / c.kv_heads);
     p.rows = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
     const long long items = (long long)c.batch * c.kv_heads * ((rows + p.rows - 1) / p.rows);
     const int len = max_len > 0 && max_len < c.rows ? max_len : c.rows;

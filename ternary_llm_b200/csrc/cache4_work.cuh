@@ -28,6 +28,13 @@ __device__ __forceinline__ float* record_of(void* ws, int ctas, int cta, int slo
 }
 #endif
 
+// New rows of a sequence: the most that the caller names, or as many as sequences have on the average.
+inline int new_rows(const Cache4& c, int tokens, int max_new)
+{
+    if (max_new <= 0) return (tokens + c.batch - 1) / c.batch;
+    return max_new < tokens ? max_new : tokens;
+}
+
 struct StepPlan {
     int rows;                                        // that go through the cache together: 4, 8 or 16
     bool whole;                                      // a tile's positions stay in one CTA

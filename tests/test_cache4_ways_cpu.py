@@ -1,0 +1,37 @@
+"""Which way a call of attention over the 4-bit cache takes, by the workspace that it asks for."""
+import ctypes
+
+import pytest
+
+import ternary_llm_b200 as tl
+from ternary_llm_b200 import _lib
+
+P = 0x10000          # an address that is never followed
+
+
+def workspace(batch, kv_heads, rows, dim, tokens, heads, max_new=0, max_len=0):
+    n = ctypes.c_size_t()
+    c = _lib.Cache4Desc(P, P, P, P, batch, kv_heads, rows, dim)
+    assert tl.lib().tllm_b200_cache4_workspace(ctypes.byref(c), tokens, heads, max_new, max_len, ctypes.byref(n)) == 0
+    return n.value
+
+
+def record(ctas, rows, dim):
+    """An entry of 32 bytes and two records of `rows` maxima, sums and outputs for each CTA."""
+    return ctas * (32 + 2 * rows * (dim + 2) * 4)
+
+
+@pytest.mark.parametrize("batch,kv_heads,rows,dim,heads", [(9, 8, 8192, 128, 32), (32, 8, 8192, 128, 32), (200, 8, 4096, 64, 32), (4096, 8, 64, 128, 32), (1, 8, 40000, 128, 32)])
+def test_single_tokens_without_a_hint(batch, kv_heads, rows, dim, heads):
+    """As with it: 4 rows of a head, in parts that are joined or in one CTA."""
+    want = 0 if rows * dim <= 160000 else record(296, 4, dim)
+    assert workspace(batch, kv_heads, rows, dim, batch, heads, 1) == want
+    assert workspace(batch, kv_heads, rows, dim, batch, heads) == want
+
+
+def test_prompts_beside_many_short_sequences_are_cut():
+    """Whole tiles would take a CTA for each tile that any of the sequences might have."""
+    assert workspace(64, 8, 4008, 128, 4063, 32, 4000) == workspace(64, 8, 4008, 128, 4063, 32) == record(148, 256, 128)
+    assert workspace(1000, 8, 2008, 128, 2999, 32, 2000) == record(148, 256, 128)
+    assert workspace(4, 8, 2008, 128, 2003, 32, 2000) == 0                   # few CTAs find nothing
+    assert workspace(1, 8, 2008, 128, 2000, 32) == 0

@@ -31,3 +31,25 @@ def test_sequences_that_share_rows(first, lens, rows, heads, kv_heads, dim):
         with pytest.raises(tl.TllmError, match="outside its tensors"):
             tl.check_device_errors()
         assert (out == 7).all()
+
+
+@pytest.mark.parametrize("before,new,heads,kv_heads,dim", [
+    ([7 * i % 3000 for i in range(32)], [1] * 32, 32, 8, 128),                             # single tokens
+    ([i % 61 for i in range(4096)], [1] * 4096, 8, 2, 64),
+    ([0] + [11 * i % 900 for i in range(40)], [500] + [1] * 40, 8, 2, 128),                # a prompt beside them
+    ([0] + [300] * 20, [1500] + [1] * 20, 32, 8, 64),
+    ([0] + [100] * 15, [1] + [20] * 15, 16, 4, 64), ([5, 900, 70], [701, 0, 300], 32, 8, 64), ([0] * 9 + [3], [0] * 9 + [130], 16, 8, 64)])
+def test_lengths_that_nobody_names(before, new, heads, kv_heads, dim):
+    """Without a number of new rows, and with the right one."""
+    gen = torch.Generator(device="cuda").manual_seed(len(new))
+    lens = [a + n for a, n in zip(before, new)]
+    c = random_cache(gen, len(new), kv_heads, max(lens), dim, lens)
+    first, lens_dev, tokens = layout(before, new)
+    some = {0, 1, 2, len(new) // 2, len(new) - 2, len(new) - 1}
+    for dtype in TYPES:
+        q = torch.randn(tokens, heads, dim, generator=gen, device="cuda").to(dtype)
+        for most in (0, max(new)):
+            out = torch.full_like(q, 7.0)
+            ops.attention(c, q, out, first, lens_dev, max_new=most)
+            tl.check_device_errors()
+            check_attention(c, q, out, before, new, heads, dtype, dim ** -0.5, some)
