@@ -15,22 +15,39 @@ static bool takes_step(const Cache4& c, int tokens, int heads, int max_new, int 
     return rows <= 32 || (tiles <= 148 && (len <= kStepWhole / c.dim || tiles * len <= 40000000 / c.dim));
 }
 
+// The way of a call: few rows, or prompts.  More units than the first can count, which a number of new rows far below the real one asks for, are
+// prompts of unknown length.
+struct Way {
+    bool few;
+    StepPlan step;
+    PromptPlan prompt;
+};
+static Way way_of(const Cache4& c, int tokens, int heads, int max_new, int max_len)
+{
+    Way w = {};
+    const int len = max_len > 0 && max_len < c.rows ? max_len : c.rows;
+    if (takes_step(c, tokens, heads, max_new, max_len)) {
+        w.step = step_plan(c, tokens, heads, max_new, max_len);
+        w.few = work_fits(c, tokens, heads, len, w.step.rows, kStepChunk, w.step.whole);
+        if (!w.few) max_new = 0;
+    }
+    if (!w.few) w.prompt = prompt_plan(c, tokens, heads, max_new, max_len);
+    return w;
+}
+
 size_t cache4_workspace(const Cache4& c, int tokens, int heads, int max_new, int max_len)
 {
     if (tokens == 0 || c.batch == 0) return 0;
-    return takes_step(c, tokens, heads, max_new, max_len) ? step_plan(c, tokens, heads, max_new, max_len).bytes : prompt_plan(c, tokens, heads, max_new, max_len).bytes;
+    const Way w = way_of(c, tokens, heads, max_new, max_len);
+    return w.few ? w.step.bytes : w.prompt.bytes;
 }
 
 template <typename T>
 int launch_cache4_attention(const Cache4Call& a, Rows<const T> q, Rows<T> out, cudaStream_t stream)
 {
     if (a.s.tokens == 0 || a.s.batch == 0) return TLLM_OK;
-    const bool step = takes_step(a.c, a.s.tokens, a.heads, a.max_new, a.max_len);
-    if (!work_fits(a, step ? 4 : 128, step ? kStepChunk : kPromptChunk))
-        return fail(TLLM_ERR_SIZE, "cache4_attention: %d rows of %d heads over %d positions", a.s.tokens, a.heads, a.c.rows);
-    if (step)
-        return launch_cache4_step<T>(a, q, out, step_plan(a.c, a.s.tokens, a.heads, a.max_new, a.max_len), stream);
-    return launch_cache4_prompt<T>(a, q, out, prompt_plan(a.c, a.s.tokens, a.heads, a.max_new, a.max_len), stream);
+    const Way w = way_of(a.c, a.s.tokens, a.heads, a.max_new, a.max_len);
+    return w.few ? launch_cache4_step<T>(a, q, out, w.step, stream) : launch_cache4_prompt<T>(a, q, out, w.prompt, stream);
 }
 
 template int launch_cache4_attention<half>(const Cache4Call&, Rows<const half>, Rows<half>, cudaStream_t);

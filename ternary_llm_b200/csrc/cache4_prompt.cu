@@ -651,6 +651,7 @@ PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int 
         p.rows = 256;
         p.whole = longest - rows * c.kv_heads * mean / 148 <= 7 && idle(256) <= 1500;
     }
+    p.whole = p.whole || !work_fits(c, tokens, heads, len, p.rows, kTile, false);
     p.ctas = p.whole ? (int)fmax(grid_of(p.rows), pairs) : 148;
     p.bytes = p.whole ? 0 : join_bytes(c.dim, p.rows, p.ctas);
     return p;

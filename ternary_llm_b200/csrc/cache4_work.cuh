@@ -35,6 +35,13 @@ inline int new_rows(const Cache4& c, int tokens, int max_new)
     return max_new < tokens ? max_new : tokens;
 }
 
+// Whether the units of a call fit 31 bits, whatever lens and a rising first hold: tiles of `rows` rows, whole or over `len` positions in chunks.
+inline bool work_fits(const Cache4& c, int tokens, int heads, int len, int rows, int chunk, bool whole)
+{
+    const double tiles = (double)tokens * (heads / c.kv_heads) / rows + c.batch, units = whole ? 1 : (double)len / chunk + 22;
+    return tiles * units * c.kv_heads < 2e9;
+}
+
 struct StepPlan {
     int rows;                                        // that go through the cache together: 4, 8 or 16
     bool whole;                                      // a tile's positions stay in one CTA
@@ -222,13 +229,6 @@ struct Work {
         set_tile(0);
     }
 };
-// Whether the units of a call fit 31 bits, whatever lens and a rising first hold.
-inline bool work_fits(const Cache4Call& a, int rows, int chunk)
-{
-    const double tiles = (double)a.s.tokens * (a.heads / a.c.kv_heads) / rows + a.c.batch, units = (double)a.s.rows / chunk + 22;
-    return tiles * units * a.c.kv_heads < 2e9;
-}
-
 template <typename T> struct Pair2;
 template <> struct Pair2<half> {
     static __device__ __forceinline__ uint32_t of(float x, float y)

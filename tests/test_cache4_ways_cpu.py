@@ -35,3 +35,11 @@ def test_prompts_beside_many_short_sequences_are_cut():
     assert workspace(1000, 8, 2008, 128, 2999, 32, 2000) == record(148, 256, 128)
     assert workspace(4, 8, 2008, 128, 2003, 32, 2000) == 0                   # few CTAs find nothing
     assert workspace(1, 8, 2008, 128, 2000, 32) == 0
+
+
+def test_more_units_than_31_bits_hold():
+    """Few rows by the hint, but far more of them: prompts of unknown length, as without the hint."""
+    assert workspace(1, 8, 131072, 64, 60000, 32, 1) == record(296, 4, 64)
+    assert workspace(1, 8, 131072, 64, 70000, 32, 1) == workspace(1, 8, 131072, 64, 70000, 32) != record(296, 4, 64)
+    # and where parts of prompts are too many, whole tiles
+    assert workspace(1, 1, 1 << 30, 64, 1000000, 1, 1000000) == 0 < workspace(1, 1, 1 << 30, 64, 1000, 1, 1000)

@@ -53,3 +53,18 @@ def test_lengths_that_nobody_names(before, new, heads, kv_heads, dim):
             ops.attention(c, q, out, first, lens_dev, max_new=most)
             tl.check_device_errors()
             check_attention(c, q, out, before, new, heads, dtype, dim ** -0.5, some)
+
+
+def test_a_long_prompt_named_as_single_tokens():
+    """Its units of few rows do not fit 31 bits: the call is taken as without the hint, and not refused."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    n, heads, kv_heads, dim = 62000, 32, 8, 64
+    c = random_cache(gen, 1, kv_heads, 131072, dim, [n])
+    q = torch.randn(n, heads, dim, generator=gen, device="cuda").half()
+    outs = [torch.full_like(q, 7.0) for _ in range(2)]
+    for most, out in zip((0, 1), outs):
+        ops.attention(c, q, out, ints(0, n), ints(n), max_new=most)
+    tl.check_device_errors()
+    assert torch.equal(*outs)
+    for i in (0, 127, 128, 30001, n - 1):                                  # rows of the prompt, each as one token behind i
+        check_attention(c, q[i:i + 1], outs[1][i:i + 1], [i], [1], heads, torch.float16, dim ** -0.5)
