@@ -15,6 +15,7 @@ tensors is at other memory, or its storage has another size.
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -24,6 +25,11 @@ from .ops import _chk, _stream
 GROUP = 64
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 SCALINGS = {"linear": 1, "ntk": 2, "yarn": 3, "llama3": 4}
+
+
+def _int(v) -> int:
+    """A whole number as an int of C holds it: the largest for one above, -1 for a negative one."""
+    return max(-1, min(operator.index(v), 2 ** 31 - 1))
 
 
 def _frequencies(rot_dim: int, base: float, scaling: dict | None):
@@ -41,7 +47,8 @@ def _frequencies(rot_dim: int, base: float, scaling: dict | None):
             (float(s.pop("low", 1.0)), float(s.pop("high", 4.0)))
     if s:
         raise ValueError(f"scaling: unknown {', '.join(map(repr, s))}")
-    f, amplitude = (ctypes.c_double * max(1, rot_dim // 2))(), ctypes.c_float()
+    rot_dim = _int(rot_dim)
+    f, amplitude = (ctypes.c_double * max(1, min(rot_dim, 512) // 2))(), ctypes.c_float()          # the library writes no more than 256
     _lib.check(_lib.lib().tllm_b200_rotary_frequencies(rot_dim, base, ctypes.byref(d), f, ctypes.byref(amplitude)))
     return f, amplitude.value
 
@@ -105,11 +112,11 @@ class RotaryTable(_Fixed):
             f, own = (ctypes.c_double * max(1, len(frequencies)))(*frequencies), 1.0
             if 2 * len(frequencies) != rot_dim:
                 raise ValueError(f"{len(frequencies)} frequencies for {rot_dim} entries")
-        self.rot_dim, self.half, self._f = rot_dim, half, f
+        self.rot_dim, self.half, self._f = rot_dim, bool(half), f
         self.amplitude = own if amplitude is None else float(amplitude)
         turns = torch.frombuffer(_turns(f, rot_dim // 2), dtype=torch.int64, count=rot_dim // 2)
         self.turns = turns.clone() if device is not None and torch.device(device).type == "cpu" else turns.to("cuda" if device is None else device)
-        self._keep(_lib.RotaryTableDesc(self.turns.data_ptr(), rot_dim, int(half), self.amplitude), self.turns)
+        self._keep(_lib.RotaryTableDesc(self.turns.data_ptr(), rot_dim, int(self.half), self.amplitude), self.turns)
 
     def __reduce__(self):
         return RotaryTable, (self.rot_dim, 0.0, self.half, None, self.frequencies, self.amplitude, str(self.turns.device))
@@ -201,7 +208,7 @@ def rotary(q, k, positions, table: RotaryTable, q_out=None, k_out=None, inverse:
             (("q", q, heads), ("q_out", q if q_out is None else q_out, heads), ("k", k, kv_heads), ("k_out", k if k_out is None else k_out, kv_heads))]
     _lib.check(_lib.lib().tllm_b200_rotary(
         kind, ctypes.byref(table._desc()), _chk(positions, torch.int32, "positions", tokens), tokens, _ref(rows[0]), _ref(rows[1]), heads,
-        _ref(rows[2]), _ref(rows[3]), kv_heads, dim, int(inverse), _stream()))
+        _ref(rows[2]), _ref(rows[3]), kv_heads, dim, int(bool(inverse)), _stream()))
 
 
 def append(cache: Cache4, q, k, v, first, lens, table: RotaryTable | None = None, q_out=None) -> None:
@@ -247,6 +254,7 @@ def attention(cache: Cache4, q, out, first, lens, scale: float | None = None, ma
     st = _lib.host().cache4_attention(cache._native, q, out, first, lens, scale, max_new, max_len)
     if st is not None:
         return _lib.check(st)
+    max_new, max_len = _int(max_new), _int(max_len)
     kind, d = _type(q, "q", (torch.float16, torch.bfloat16)), cache._desc()
     tokens, heads = q.shape[:2]
     x, y = _rows(q, q.dtype, "q", tokens, heads, cache.dim), _rows(out, q.dtype, "out", tokens, heads, cache.dim)

@@ -162,3 +162,54 @@ def test_a_handle_of_tensors_without_memory():
     t[3].untyped_storage().resize_(16)
     with pytest.raises(ValueError, match="storage"):
         ops.Cache4(*t)
+
+
+class Library:
+    """Functions of the C ABI that write down their whole numbers, converted as the ABI has them."""
+
+    def __init__(self):
+        self.calls = []
+        signatures = _lib.SIGNATURES
+        for name in ("tllm_b200_cache4_workspace", "tllm_b200_cache4_attention", "tllm_b200_rotary"):
+            types = signatures[name][1]
+            setattr(self, name, ctypes.CFUNCTYPE(INT, *types)(lambda *a, name=name: self.calls.append((name, a)) or 0))
+
+
+@pytest.mark.parametrize("max_new,max_len,want", [
+    (1, 2 ** 32 + 5, (1, 2 ** 31 - 1)), (2 ** 32 + 1, 7, (2 ** 31 - 1, 7)), (2 ** 31, 2 ** 40, (2 ** 31 - 1, 2 ** 31 - 1)), (3, 4, (3, 4)), (-2 ** 32, 0, (-1, 0)),
+    (0, -2 ** 32 + 9, (0, -1)), (True, 4, (1, 4))])
+def test_hints_beyond_32_bits(seen, monkeypatch, max_new, max_len, want):
+    """A limit that no int holds is none, and a negative one stays what the library refuses."""
+    c, _, _ = make()
+    x, first, lens = on_device(3, 2, 64, dtype=torch.float16), on_device(3, dtype=torch.int32), on_device(2, dtype=torch.int32)
+    library = Library()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(ops, "_stream", lambda: None)
+    monkeypatch.setattr(ops._lib, "lib", lambda: library)
+    ops.attention(c, x, x.clone().as_subclass(OnDevice), first, lens, scale=1, max_new=max_new, max_len=max_len)      # a scale that is no float goes the other way
+    (_, w), (_, a) = library.calls
+    assert w[3:5] == a[9:11] == want
+    with pytest.raises(TypeError):
+        ops.attention(c, x, x.clone().as_subclass(OnDevice), first, lens, max_len=7.5)
+
+
+@pytest.mark.parametrize("rot", [-2 ** 32 + 64, 2 ** 31])
+def test_head_parts_beyond_32_bits(rot):
+    with pytest.raises(_lib.TllmError, match="rot_dim"):
+        ops.rotary_frequencies(rot, 1e4)
+    with pytest.raises(_lib.TllmError, match="rot_dim"):
+        ops.RotaryTable(rot, 1e4, device="cpu")
+
+
+def test_layout_and_direction_are_truth_values(seen, monkeypatch):
+    _, t, _ = make()
+    library = Library()
+    x = on_device(3, 2, 64, dtype=torch.float16)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    monkeypatch.setattr(ops, "_stream", lambda: None)
+    monkeypatch.setattr(ops._lib, "lib", lambda: library)
+    for inverse in (2 ** 32, 1, 0):
+        ops.rotary(x, None, on_device(3, dtype=torch.int32), t, inverse=inverse)
+    assert [a[12] for _, a in library.calls] == [1, 1, 0]
+    monkeypatch.undo()
+    assert _lib.RotaryTableDesc.from_buffer_copy(ops.RotaryTable(64, half=2 ** 32, device="cpu")._native[0]).half_layout == 1
