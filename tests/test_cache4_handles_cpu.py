@@ -210,6 +210,6 @@ def test_layout_and_direction_are_truth_values(seen, monkeypatch):
     monkeypatch.setattr(ops._lib, "lib", lambda: library)
     for inverse in (2 ** 32, 1, 0):
         ops.rotary(x, None, on_device(3, dtype=torch.int32), t, inverse=inverse)
-    assert [a[12] for _, a in library.calls] == [1, 1, 0]
+    assert [a[11] for _, a in library.calls] == [1, 1, 0]
     monkeypatch.undo()
     assert _lib.RotaryTableDesc.from_buffer_copy(ops.RotaryTable(64, half=2 ** 32, device="cpu")._native[0]).half_layout == 1
