@@ -99,7 +99,7 @@ int tllm_b200_rotary(int type, const tllm_b200_rotary_table* table, const int* p
     if (!table || (!positions && tokens > 0)) return fail(TLLM_ERR_NULL, "rotary: null pointer");
     int st = check_type(fn, type, true);
     if (st) return st;
-    if (tokens < 0 || tokens > kMostTokens || heads < 1 || kv_heads < 0 || heads > kMostHeads || kv_heads > kMostHeads || dim < 8 || dim > 512 || dim * type_size(type) % 16)
+    if (tokens < 0 || tokens > kMostTokens || heads < 1 || kv_heads < 0 || heads > kMostHeads || kv_heads > kMostHeads || dim < 4 || dim > 512 || dim * type_size(type) % 16)
         return fail(TLLM_ERR_SHAPE, "rotary: tokens=%d heads=%d/%d dim=%d", tokens, heads, kv_heads, dim);
     if ((k != nullptr) != (kv_heads > 0) || (k != nullptr) != (k_out != nullptr)) return fail(TLLM_ERR_NULL, "rotary: k, k_out and kv_heads go together");
     Rotary r;

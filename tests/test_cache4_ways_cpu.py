@@ -43,3 +43,11 @@ def test_more_units_than_31_bits_hold():
     assert workspace(1, 8, 131072, 64, 70000, 32, 1) == workspace(1, 8, 131072, 64, 70000, 32) != record(296, 4, 64)
     # and where parts of prompts are too many, whole tiles
     assert workspace(1, 1, 1 << 30, 64, 1000000, 1, 1000000) == 0 < workspace(1, 1, 1 << 30, 64, 1000, 1, 1000)
+
+
+@pytest.mark.parametrize("type,dim,fits", [(2, 4, True), (2, 8, True), (2, 2, False), (0, 4, False), (1, 4, False), (0, 8, True), (2, 512, True), (2, 516, False)])
+def test_head_sizes_of_rotary(type, dim, fits):
+    """A multiple of 8, of 4 for FP32, up to 512; what is refused is refused before the device is looked for."""
+    x, t = ctypes.byref(_lib.HeadsDesc(P, 2 * dim)), ctypes.byref(_lib.RotaryTableDesc(P, 2, 1, 1.0))
+    status = tl.lib().tllm_b200_rotary(type, t, P, 0, x, x, 2, None, None, 0, dim, 0, None)
+    assert (status != -3) == fits, tl.lib().tllm_b200_last_error()

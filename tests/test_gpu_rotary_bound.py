@@ -40,3 +40,18 @@ def test_angles_are_64_bits(dtype, half, dim, rot, tokens, start, inverse):
     err = np.abs(f64(y) - want)
     assert (err[..., :rot] <= bound[..., :rot]).all(), float((err / bound)[..., :rot].max())
     assert (f64(y)[..., rot:] == v[..., rot:]).all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rot", [2, 4])
+@pytest.mark.parametrize("tokens,heads", [(1, 1), (5, 33), (700, 40)])
+def test_the_smallest_head(half, rot, tokens, heads):
+    """16 bytes: four FP32 numbers."""
+    gen = torch.Generator(device="cuda").manual_seed(rot)
+    table = ops.RotaryTable(rot, 1e4, half=half)
+    x = torch.randn(tokens, heads, 4, generator=gen, device="cuda")
+    position, y = torch.arange(tokens, dtype=torch.int32, device="cuda"), torch.empty_like(x)
+    ops.rotary(x, None, position, table, y)
+    v = f64(x)
+    want = ref.rotate(v, np.arange(tokens), table.frequencies, 1.0, half)
+    assert (np.abs(f64(y) - want) <= 2.0 ** -24 * np.abs(want) + 3.01 * 2.0 ** -24 * 2 * np.abs(v).max(-1, keepdims=True)).all()
