@@ -9,7 +9,9 @@
  * Cache.  Codes uint8 [batch, kv_heads, rows, dim / 2] and params half [batch, kv_heads, rows, dim / 64, 2],
  * for keys and for values.  64 neighbouring values share (s, l): value = s c + l, c = 0..15.  Eight
  * neighbouring values lie in 32 bits: value 2 i in nibble i, value 2 i + 1 in nibble i + 4.  Position p of
- * sequence b is row p of entry b.  A cache that a caller fills may have scales of either sign.
+ * sequence b is row p of entry b.  A cache that a caller fills may have scales of either sign; its params are
+ * finite and s c + l of every code within FP16's range, as append leaves them, or a key's are NaN, which marks its
+ * position.  (Attention of many rows holds s c + l as FP16: beyond 65504 it would be infinite there alone.)
  *
  * Sequences of a call.  Activations are [tokens, heads, dim]; sequence b has their rows first[b] ..
  * first[b + 1] - 1 (int [batch + 1] on the device, rising) and holds lens[b] positions (int [batch] on the

@@ -130,7 +130,8 @@ class RotaryTable(_Fixed):
 
 
 class Cache4(_Fixed):
-    """Codes uint8 [batch, kv_heads, rows, dim / 2] and params float16 [batch, kv_heads, rows, dim / 64, 2] of keys and values."""
+    """Codes uint8 [batch, kv_heads, rows, dim / 2] and params float16 [batch, kv_heads, rows, dim / 64, 2] of keys and values.
+    Params that append did not write: finite, of either sign, and s c + l of every code within FP16's range."""
 
     def __init__(self, k_codes, k_params, v_codes, v_params):
         if k_codes.dim() != 4:
@@ -247,8 +248,9 @@ def read(cache: Cache4, k, v, first, lens) -> None:
 
 def attention(cache: Cache4, q, out, first, lens, scale: float | None = None, max_new: int = 0, max_len: int = 0) -> None:
     """out = softmax(scale q k') v over the positions up to each row's own (scale: dim ** -0.5).  max_new: about the most rows
-    of a sequence, 0 where the caller does not know; results do not depend on it but for the order of sums.  max_len: no
-    sequence holds more positions (0: the cache's rows); workspaces are as large as that needs.  FP16 or BF16."""
+    of a sequence, 0 where the caller does not know (then their average); it chooses the way of the work, and ways differ in
+    the order of sums and in what they round to 11 bits.  max_len: no sequence holds more positions (0: the cache's rows);
+    workspaces are as large as that needs.  FP16 or BF16."""
     if scale is None:
         scale = cache.dim ** -0.5
     st = _lib.host().cache4_attention(cache._native, q, out, first, lens, scale, max_new, max_len)
