@@ -4,15 +4,16 @@
 
 namespace tllm {
 
-// Rows of a key/value head go 16 at once through mma.sync up to 32 of them, and while a tile of 16 a SM takes the call and its positions are few;
-// behind that 128 or 256 at once through tcgen05.  Both sides, us, 32 heads over 8: of 64, 14 sequences of 4 tokens behind 6000 31 / 73, one of 64
-// behind 2500 23.7 / 24.6, behind 6000 34 / 28; of 128, one of 40 (80 tiles) behind 2500 24 / 29, behind 6000 35 / 33, one of 64 (128) behind
-// 300 9.3 / 14.3, behind 6000 49 / 34, 14 of 9 (336) behind 300 22 / 14, behind 2500 60 / 47.
+// Rows of a key/value head go 16 at once through mma.sync up to 32 of them, and while a tile of 16 an SM takes the call and stays in one CTA; behind
+// that 128 or 256 at once through tcgen05.  Both sides, us, 32 heads over 8, caches beyond L2 in turn: of 128, one sequence of 64 tokens behind 700
+// 12.5 / 16.4, of 40 behind 1200 15.8 / 19.5, behind 1800 23.0 / 19.8, of 64 behind 6000 51.8 / 26.1, 14 of 9 (336 tiles) behind 300 24.1 / 11.9; of 64,
+// one of 64 behind 2400 about equal, behind 6000 35.5 / 22.0.  Up to 32 rows: 14 of 4 behind 6000 47.6 / 77.2, 6 of 5 behind 2500 27.3 / 24.2, of 64
+// 32.9 / 64.1 and 20.4 / 21.2.
 static bool takes_step(const Cache4& c, int tokens, int heads, int max_new, int max_len)
 {
     const long long rows = (long long)new_rows(c, tokens, max_new) * (heads / c.kv_heads);
     const long long tiles = (rows + 15) / 16 * c.batch * c.kv_heads, len = max_len > 0 && max_len < c.rows ? max_len : c.rows;
-    return rows <= 32 || (tiles <= 148 && (len <= kStepWhole / c.dim || tiles * len <= 40000000 / c.dim));
+    return rows <= 32 || (tiles <= 148 && len <= kStepWhole / c.dim);
 }
 
 // The way of a call: few rows, or prompts.  More units than the first can count, which a number of new rows far below the real one asks for, are

@@ -636,8 +636,8 @@ PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int 
     if (tiles_of(128) <= 148) {
         // An SM for each tile of 128 rows: the quickest of these tiles whole, cut, and tiles of 256 rows cut, as they measure, us: 8 + 1.9 for each
         // tile of positions, or 19 + 1.85 for each that a CTA takes, or 27 + 2.35; sequences of a batch differ, so that cut ones have fewer.
-        // 32 heads of 128 over 8, one sequence: 79 tokens behind 500 18.6 / 25.0 / 25.9, behind 2500 50.1 / 27.3 / 35.7, behind 16000 243 / 64 /
-        // 61; 500 behind 1200 36.4 / 48.2 / 42.0, behind 6000 111 / 117 / 85.  Tiles of 256 whole take 22.0, 60.9, 297, 42.8 and 131.
+        // 32 heads of 128 over 8, one sequence: 79 tokens behind 500 15.1 / 20.4 / 24.8, behind 2500 40.7 / 21.6 / 27.8, behind 16000 209 / 51 /
+        // 54; 500 behind 1200 30.4 / 40.2 / 38.2, behind 6000 90 / 95 / 75.  Tiles of 256 whole take 18.7, 52.2, 268, 37.2 and 116.
         const double few = c.batch > 1 ? 0.85 : 1;
         const auto cut = [&](int rows) { return fmax(tiles_of(rows) * (few * mean + Work<128, kTile>::kFixed) / 148, (double)Work<128, kTile>::kLeast); };
         const double whole = 8 + 1.9 * longest + idle(128) / 75, halves = 19 + 1.85 * cut(128), full = 27 + 2.35 * cut(256);
@@ -646,7 +646,7 @@ PromptPlan prompt_plan(const Cache4& c, int tokens, int heads, int max_new, int 
     } else {
         // A tile of rows stays in one CTA unless the longest would keep its SM busy for more than seven tiles of positions (some 2 us each) after
         // the others are done, which is what cutting costs in records and a second launch.  Both ways, us, 32 heads over 8: of 128, a prompt of
-        // 1500 39 whole, 57 cut, 2000 52 / 74; of 64, four prompts of 700 38 / 51.
+        // 1500 34 whole, 50 cut, 2000 48 / 69; of 64, four prompts of 700 34 / 43.
         const double rows = (double)tokens * per / 256 > (double)c.batch ? (double)tokens * per / 256 : (double)c.batch;
         p.rows = 256;
         p.whole = longest - rows * c.kv_heads * mean / 148 <= 7 && idle(256) <= 1500;

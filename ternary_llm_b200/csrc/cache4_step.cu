@@ -554,13 +554,13 @@ StepPlan step_plan(const Cache4& c, int tokens, int heads, int max_new, int max_
     const long long items = (long long)c.batch * c.kv_heads * ((rows + p.rows - 1) / p.rows);
     const int len = max_len > 0 && max_len < c.rows ? max_len : c.rows;
     // A tile's positions stay in one CTA while that takes no longer than a second launch and what it waits for.  Both ways, us, one / 48
-    // sequences of 32 heads over 8: heads of 128 behind 300 6.4 / 14.2 in one CTA, 12.1 / 17.2 cut; behind 800 8.8 / 20.1, 12.7 / 24.3; behind
-    // 1200 10.3 / 24.0, 12.4 / 27.6; behind 2000 13.7 / 34.0, 11.4 / 37.5; heads of 64 behind 2000 9.3 / 21.5, 9.5 / 25.3.
+    // sequences of 32 heads over 8, caches beyond L2 in turn: heads of 128 behind 300 6.3 / 15.3 in one CTA, 12.1 / 18.5 cut; behind 800 9.3 / 21.2, 12.3 /
+    // 23.9; behind 1200 10.9 / 24.9, 12.8 / 27.9; behind 2000 14.5 / 34.2, 13.1 / 36.4; heads of 64 behind 2000 9.4 / 21.6, 11.1 / 24.1.
     p.whole = len <= kStepWhole / c.dim;
     // More than two such rounds of CTAs: one round, each with an equal number of tiles in a row, which saves what a CTA does before its first
     // tile, and costs where lengths differ.  One token each, 32 heads of 128 over 8, up to 800 positions, us, one round / a CTA a tile: equal
-    // lengths 48 sequences 22.2 / 20.4, 96 33.7 / 36.2, 256 76.9 / 97.9; lengths between 1 and that 20.5 / 16.6, 30.0 / 27.6, 69.5 / 77.3;
-    // 1024 of 8 heads over one 59 / 91.
+    // lengths 48 sequences 21.3 / 20.1, 96 31.9 / 35.0, 256 72.1 / 92.2; lengths between 1 and that 21.4 / 19.0, 29.9 / 27.3, 64.4 / 76.0;
+    // 1024 of 8 heads over one 70 / 102.
     const int round = p.rows == 16 ? 148 : 296;
     p.ctas = p.whole && items <= 2 * round ? (int)items : round;
     p.bytes = p.whole ? 0 : join_bytes(c.dim, p.rows, p.ctas);

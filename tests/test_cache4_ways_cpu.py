@@ -51,3 +51,10 @@ def test_head_sizes_of_rotary(type, dim, fits):
     x, t = ctypes.byref(_lib.HeadsDesc(P, 2 * dim)), ctypes.byref(_lib.RotaryTableDesc(P, 2, 1, 1.0))
     status = tl.lib().tllm_b200_rotary(type, t, P, 0, x, x, 2, None, None, 0, dim, 0, None)
     assert (status != -3) == fits, tl.lib().tllm_b200_last_error()
+
+
+def test_many_tiles_of_few_rows_stay_in_one_cta():
+    """33 rows of a head and more are prompts where a tile of 16 would be cut."""
+    assert workspace(1, 8, 1250, 128, 40, 32, 40) == 0 == workspace(1, 8, 2500, 64, 64, 32, 64)
+    assert workspace(1, 8, 2541, 128, 40, 32, 40) == record(148, 128, 128) and workspace(1, 8, 6000, 64, 64, 32, 64) == record(148, 128, 64)
+    assert workspace(1, 8, 2541, 128, 8, 32, 8) == record(148, 16, 128)

@@ -84,7 +84,7 @@ FOUR, EIGHT, SIXTEEN, TILES, PAIRS = (296, 4), (296, 8), (148, 16), (148, 128), 
     ([131000], [1], 8, 2, 128, FOUR), ([0, 30000, 31, 32, 33, 12345], [1] * 6, 8, 2, 64, FOUR),
     ([20000], [1], 8, 1, 64, EIGHT), ([2600, 40, 7000], [2, 1, 2], 32, 8, 128, EIGHT), ([5000 + 311 * i for i in range(12)], [1] * 12, 35, 5, 64, EIGHT),
     ([20000], [1], 16, 1, 64, SIXTEEN), ([1300, 2900, 1777], [5, 3, 1], 32, 8, 128, SIXTEEN), ([4001, 17, 9000], [4, 2, 3], 12, 4, 64, SIXTEEN),
-    ([3000], [64], 2, 2, 128, SIXTEEN), ([2990, 0], [31, 32], 1, 1, 64, SIXTEEN),
+    ([3000], [32], 2, 2, 128, SIXTEEN), ([2990, 0], [31, 32], 1, 1, 64, SIXTEEN),
     ([300], [1], 32, 8, 128, None), ([31 * i for i in range(40)], [1 + i % 2 for i in range(40)], 16, 8, 64, None), ([700], [32], 3, 3, 128, None)])
 @pytest.mark.parametrize("size", [0.0, 1.0])
 def test_few_rows(dtype, before, new, heads, kv_heads, dim, way, size):
