@@ -3,8 +3,9 @@
 //
 // A CTA here for each that has the first chunk of a shared tile: weights of all records first, then their outputs, every
 // load independent of the others.  A thread has four channels of a row and every kParts-th record; the parts meet in
-// shared memory.  The order of all sums is fixed.  Bound by three dependent rounds of loads and the launch: some 4 us
-// for 296 records of 4 rows of 128, whose 0.6 MB come from L2.
+// shared memory.  The order of all sums is fixed.  Bound by three dependent rounds of loads and the launch: alone, with records in L2, 6.4 us
+// for 296 records of 4 rows of 128, 37 a tile (0.6 MB; 8.7 from DRAM), 4.6 where 300 tiles are shared by one to ten, 13.9 for 148 of 256 rows
+// (27 MB; 19 from DRAM).
 #include "cache4.cuh"
 #include "cache4_work.cuh"
 #include "dense.cuh"
