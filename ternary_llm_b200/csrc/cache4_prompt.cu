@@ -7,7 +7,7 @@
 //   S = Q K^T    128 FP32 columns of tensor memory for each tile of rows; keys in shared memory, queries too, or for heads
 //                of 64, where it has room, in tensor memory (nine prompts 3 % quicker)
 //   softmax      a thread reads its row; the weights go back over S as FP16, with a factor of 2^6 that leaves small
-//                ones their bits (the sum of the weights takes it out)
+//                ones their bits (the sum of the weights takes it out): 11 of them down to 2^-20 of the largest, steps of 2^-30 of it below
 //   O += P V     weights from tensor memory, values feature-major
 // so a tile of the cache is unpacked once for 256 rows, and one tile's products run beside the other's softmax.
 // BF16 queries become FP16 numbers times a power of two of their row.  The running maximum moves when a score exceeds it
