@@ -18,7 +18,7 @@
 // every CTA takes an equal part, parts of a tile of rows joined by a second launch in their order.
 // All mbarrier waits are bounded.
 //
-// What bounds it: 512 tokens of 32 heads of 128 over 8 behind 16000 take 149 - 168 us by the box, 0.81 - 0.92 PFLOP/s (the power
+// What bounds it: 512 tokens of 32 heads of 128 over 8 behind 16000 take 149 - 168 us from card to card, 0.81 - 0.92 PFLOP/s (the power
 // limit decides), 14 of them the join; 149 were 136 without the exponentials, and 158, before the scores were read twice, 125 without any softmax
 // arithmetic and 149 without the products: the softmax warps, then the tensor pipe.  Heads of 64 have half the products for the same
 // softmax: nine prompts of 4529 tokens in all take 115, 99 without the exponentials, of which 28 are their full rate.
